@@ -12,6 +12,7 @@ LIB_PATH = os.environ.get(
 
 _c = ctypes
 _i64, _i32, _f32, _vp, _int = _c.c_int64, _c.c_int32, _c.c_float, _c.c_void_p, _c.c_int
+_f64 = _c.c_double
 
 # name -> (restype, argtypes); mirrors include/incagg_gnn.h one to one.
 SIGNATURES = {
@@ -60,6 +61,19 @@ SIGNATURES = {
     "incagg_softmax_xent_forward_f32": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp]),
     "incagg_softmax_xent_backward_f32": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
     "incagg_adam_step_f32": (_int, [_vp, _i64, _f32, _f32, _f32, _f32, _f32, _vp]),
+    "incagg_grad_norm_ws_doubles": (_i64, [_i64, _i64]),
+    "incagg_grad_norm": (_int, [_vp, _i64, _int, _vp, _i64, _vp, _vp]),
+    "incagg_grad_clip": (_int, [_vp, _i64, _int, _f64, _vp, _i64, _vp, _vp]),
+    "incagg_adam_step_clipped_f32": (_int, [_vp, _i64, _vp, _i64, _f64, _vp, _i64, _vp, _vp]),
+    "incagg_group_rows_max_groups": (_i64, []),
+    "incagg_group_rows_ws_ints": (_i64, [_i64, _i64]),
+    "incagg_group_rows": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "incagg_group_ptr": (_int, [_vp, _int, _i64, _i64, _vp, _vp]),
+    "incagg_grouped_gemm": (_int, [_vp, _i64, _vp, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64,
+                                   _i64, _i64, _i64, _int, _vp, _i64, _vp]),
+    "incagg_grouped_tn_ws_bytes": (_i64, [_i64, _i64, _i64, _i64, _int]),
+    "incagg_grouped_tn": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp,
+                                 _i64, _vp, _vp, _i64, _vp]),
     "incagg_gather_rows_f32": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
     "incagg_scatter_rows_f32": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
     "incagg_copy_row_chunks_f32": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp,
@@ -93,12 +107,17 @@ class SpmmFuseStruct(_c.Structure):
 
 
 REDUCE = {"sum": 0, "add": 0, "mean": 1}
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 
 class AdamSegment(_c.Structure):
     """``incagg_adam_segment`` of include/incagg_gnn.h."""
     _fields_ = [("p", _vp), ("g", _vp), ("m", _vp), ("v", _vp), ("step", _vp), ("n", _i64)]
+
+
+class AdamHyper(_c.Structure):
+    """``incagg_adam_hyper`` of include/incagg_gnn.h."""
+    _fields_ = [(name, _f64) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
 
 
 class SpmmPlanStruct(_c.Structure):

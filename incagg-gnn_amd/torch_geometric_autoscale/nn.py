@@ -548,6 +548,68 @@ class RowsLinear(Linear):
         return _RowsLinear.apply(x, self.weight, self.bias, self.gathered)
 
 
+class _GroupedLinear(torch.autograd.Function):
+    """``y[i] = x[i] @ W[g(i)]^T + b[g(i)]`` over rows of several groups."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, gathered):
+        ctx.save_for_backward(x, weight)
+        ctx.groups, ctx.has_bias = groups, bias is not None
+        ctx.gathered = gathered and x.dtype == torch.float32
+        out = ops.rows_empty(x.size(0), weight.size(1), x.device) if ctx.gathered else None
+        return ops.grouped_gemm(x, weight, groups, trans_w=True, bias=bias, out=out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        need, groups = ctx.needs_input_grad, ctx.groups
+        dx = dw = db = None
+        if need[0]:
+            out = ops.rows_empty(x.size(0), x.size(1), x.device) if ctx.gathered else None
+            dx = ops.grouped_gemm(dy, weight, groups, out=out)
+        if need[1] or (ctx.has_bias and need[2]):
+            with_bias = ctx.has_bias and need[2]
+            dw = ops.grouped_tn(dy, x, groups, column_sums=with_bias)
+            if with_bias:
+                dw, db = dw
+        return dx, dw if need[1] else None, db, None, None
+
+
+def grouped_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], groups: "ops.RowGroups",
+                   gathered: bool = False) -> Tensor:
+    """``x[i] @ weight[g]^T + bias[g]`` for every row ``i``, ``g`` its group (``groups``:
+    ops.group_rows / ops.groups_from_ptr); ``weight``: [n_groups, out, in], ``bias``:
+    [n_groups, out] or ``None``.  Rows of no group give zeros, and get zero gradients.
+    ``gathered``: a float32 result gets the row pitch an aggregation wants of its source."""
+    return _GroupedLinear.apply(x, weight, bias, groups, bool(gathered))
+
+
+class GroupedLinear(torch.nn.Module):
+    """One ``torch.nn.Linear`` per group of rows (node types of a heterogeneous graph, experts):
+    ``weight`` [n_groups, out, in] and ``bias`` [n_groups, out], each group initialised as a Linear
+    of its own.  ``groups`` says which rows are whose and is built once per batch
+    (ops.group_rows).  ``gathered``: see :class:`RowsLinear`.  GPU only, like the aggregations."""
+
+    def __init__(self, in_features: int, out_features: int, n_groups: int, bias: bool = True,
+                 gathered: bool = True):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        self.n_groups, self.gathered = n_groups, gathered
+        self.weight = Parameter(torch.empty(n_groups, out_features, in_features))
+        self.bias = Parameter(torch.empty(n_groups, out_features)) if bias else None
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        bound = 1.0 / math.sqrt(self.in_features) if self.in_features > 0 else 0.0
+        torch.nn.init.uniform_(self.weight, -bound, bound)
+        if self.bias is not None:
+            torch.nn.init.uniform_(self.bias, -bound, bound)
+
+    def forward(self, x: Tensor, groups: "ops.RowGroups") -> Tensor:
+        return grouped_linear(x, self.weight, self.bias, groups, self.gathered)
+
+
 def glorot_(w: Tensor) -> None:
     a = math.sqrt(6.0 / (w.size(-2) + w.size(-1)))
     with torch.no_grad():

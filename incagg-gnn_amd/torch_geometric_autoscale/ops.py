@@ -730,6 +730,159 @@ def softmax_cross_entropy(logits: Tensor, labels: Tensor) -> Tensor:
     return _SoftmaxXent.apply(logits, labels)
 
 
+# --------------------------------------------------------------------------- rows of several kinds
+DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # INCAGG_DTYPE_*
+
+
+class RowGroups:
+    """Which rows belong to which group (node type, expert, partition): ``order`` (int32 [rows];
+    ``None``: the rows lie sorted already) lists the row numbers group by group, rows of no group
+    last; group ``g`` is ``order[ptr[g]:ptr[g + 1]]`` (int32 [n_groups + 1]).  A pure function of
+    the rows' kinds, built by :func:`group_rows` or :func:`groups_from_ptr` once per batch and
+    passed to every grouped product over those rows.  The sizes of the groups stay on the GPU:
+    nothing here waits for it."""
+
+    def __init__(self, order: Optional[Tensor], ptr: Tensor, n_rows: int):
+        self.order, self.ptr, self.n_rows = order, ptr, int(n_rows)
+        self.n_groups = ptr.numel() - 1
+
+    @property
+    def device(self):
+        return self.ptr.device
+
+
+def _max_groups(n_groups: int) -> int:
+    n_groups = int(n_groups)
+    limit = lib().incagg_group_rows_max_groups()
+    if not 1 <= n_groups <= limit:
+        raise ValueError(f"n_groups must be between 1 and {limit}, got {n_groups}")
+    return n_groups
+
+
+def _group_index(t: Tensor, name: str) -> None:
+    if t.dtype not in (torch.int64, torch.int32) or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous 1-D int64 or int32 tensor")
+
+
+def group_rows(ids: Tensor, n_groups: int) -> RowGroups:
+    """Rows ordered by the group ``ids[i]`` in ``[0, n_groups)`` each of them belongs to, equal
+    ids in row order; ``-1``: the row has no group (incagg_group_rows).  Ids outside
+    ``[-1, n_groups)`` are reported by ``check_device_errors``; their rows have no group."""
+    _need_cuda(ids, "ids")
+    _group_index(ids, "ids")
+    n_groups, rows, dev = _max_groups(n_groups), ids.numel(), ids.device
+    L = lib()
+    need = L.incagg_group_rows_ws_ints(rows, n_groups)
+    check(need)
+    order = torch.empty(rows, dtype=torch.int32, device=dev)
+    ptr = torch.empty(n_groups + 1, dtype=torch.int32, device=dev)
+    ws = torch.empty(need, dtype=torch.int32, device=dev) if need else None
+    with _on_device(dev):
+        check(L.incagg_group_rows(_ptr(ids), 1 if ids.dtype == torch.int64 else 0, rows, n_groups,
+                                  _ptr(ws), need, _ptr(order), ptr.data_ptr(), _stream_of(dev)))
+    return RowGroups(order, ptr, rows)
+
+
+def groups_from_ptr(ptr: Tensor, n_rows: int) -> RowGroups:
+    """Groups of rows that lie sorted already: group ``g`` is rows ``[ptr[g], ptr[g + 1])``, rows
+    from ``ptr[-1]`` on have no group (incagg_group_ptr).  ``ptr[0]`` is 0; entries that descend or
+    pass ``n_rows`` are reported by ``check_device_errors`` and moved to the nearest allowed
+    value."""
+    _need_cuda(ptr, "ptr")
+    _group_index(ptr, "ptr")
+    n_groups, n_rows, dev = _max_groups(ptr.numel() - 1), int(n_rows), ptr.device
+    out = torch.empty(n_groups + 1, dtype=torch.int32, device=dev)
+    with _on_device(dev):
+        check(lib().incagg_group_ptr(ptr.data_ptr(), 1 if ptr.dtype == torch.int64 else 0, n_groups,
+                                     n_rows, out.data_ptr(), _stream_of(dev)))
+    return RowGroups(None, out, n_rows)
+
+
+def _grouped_rows(t: Tensor, name: str, groups: RowGroups, dtype=None) -> None:
+    _need_cuda(t, name)
+    if t.dtype not in DTYPE_CODE or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"{name} must be " + (str(dtype) if dtype is not None else
+                        "float32, bfloat16 or float16") + f", got {t.dtype}")
+    if t.dim() != 2 or t.size(0) != groups.n_rows:
+        raise ValueError(f"{name} must be [{groups.n_rows}, width], got {tuple(t.shape)}")
+    if t.device != groups.device:
+        raise ValueError(f"{name} is on {t.device}, the groups are on {groups.device}")
+    if t.size(1) < 1:
+        raise ValueError(f"{name} has no columns")
+
+
+def _plain_rows(t: Tensor) -> Tensor:
+    """``t``, or a copy of it where its rows are not unit-stride or overlap (an expanded
+    gradient)."""
+    if (t.size(1) > 1 and t.stride(1) != 1) or (t.size(0) > 1 and t.stride(0) < t.size(1)):
+        return t.contiguous()
+    return t
+
+
+def grouped_gemm(x: Tensor, w: Tensor, groups: RowGroups, trans_w: bool = False,
+                 bias: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
+    """``y[i] = x[i] @ W[g] + bias[g]`` with ``g`` the group of row ``i`` (incagg_grouped_gemm);
+    ``w``: [n_groups, k, n], or [n_groups, n, k] with ``trans_w`` (``y = x @ W[g]^T``).  Rows of no
+    group give zeros.  float32, bfloat16 or float16, all operands alike; float32 sums."""
+    _grouped_rows(x, "x", groups)
+    dev, dt = x.device, x.dtype
+    if w.dtype != dt or (bias is not None and bias.dtype != dt):
+        raise TypeError(f"x, w and bias must have one dtype, got {dt}, {w.dtype}"
+                        + ("" if bias is None else f", {bias.dtype}"))
+    if w.dim() != 3 or w.size(0) != groups.n_groups or w.size(2 if trans_w else 1) != x.size(1):
+        raise ValueError(f"w must be [{groups.n_groups}, "
+                         + ("n, " if trans_w else "") + f"{x.size(1)}"
+                         + ("" if trans_w else ", n") + f"], got {tuple(w.shape)}")
+    n = w.size(1 if trans_w else 2)
+    if n < 1:
+        raise ValueError("w has no columns")
+    if w.device != dev or (bias is not None and bias.device != dev):
+        raise ValueError("x, w and bias must be on one device")
+    if bias is not None and tuple(bias.shape) != (groups.n_groups, n):
+        raise ValueError(f"bias must be [{groups.n_groups}, {n}], got {tuple(bias.shape)}")
+    x = _plain_rows(x)
+    if w.stride(2) != 1 or w.stride(1) < w.size(2) or w.stride(0) < 0:
+        w = w.contiguous()
+    if bias is not None and (bias.stride(1) != 1 or bias.stride(0) < n):
+        bias = bias.contiguous()
+    if out is None:
+        out = torch.empty((x.size(0), n), dtype=dt, device=dev)
+    else:
+        _grouped_rows(out, "out", groups, dt)
+        if out.size(1) != n or _plain_rows(out) is not out:
+            raise ValueError(f"out must be [{x.size(0)}, {n}] with unit-stride rows")
+    with _on_device(dev):
+        check(lib().incagg_grouped_gemm(
+            _ptr(x), _ld(x), _ptr(w), w.stride(1), w.stride(0), 1 if trans_w else 0, _ptr(bias),
+            0 if bias is None else bias.stride(0), groups.ptr.data_ptr(), _ptr(groups.order),
+            groups.n_groups, groups.n_rows, x.size(1), n, DTYPE_CODE[dt], _ptr(out), _ld(out),
+            _stream_of(dev)))
+    return out
+
+
+def grouped_tn(a: Tensor, b: Tensor, groups: RowGroups, column_sums: bool = False):
+    """``d[g] = sum over the rows i of group g of a[i]^T b[i]`` -- [n_groups, m, n], zeros for a
+    group without rows -- and with ``column_sums`` also the sums of those ``a[i]``, [n_groups, m]
+    (incagg_grouped_tn): the weight and bias gradients of :func:`grouped_gemm`.  The same bits every
+    time."""
+    _grouped_rows(a, "a", groups)
+    _grouped_rows(b, "b", groups, a.dtype)
+    a, b = _plain_rows(a), _plain_rows(b)
+    dev, dt, m, n = a.device, a.dtype, a.size(1), b.size(1)
+    L = lib()
+    need = L.incagg_grouped_tn_ws_bytes(groups.n_groups, groups.n_rows, m, n, DTYPE_CODE[dt])
+    check(need)
+    d = torch.empty((groups.n_groups, m, n), dtype=dt, device=dev)
+    sums = torch.empty((groups.n_groups, m), dtype=dt, device=dev) if column_sums else None
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _on_device(dev):
+        check(L.incagg_grouped_tn(
+            _ptr(a), _ld(a), _ptr(b), _ld(b), groups.ptr.data_ptr(), _ptr(groups.order),
+            groups.n_groups, groups.n_rows, m, n, DTYPE_CODE[dt], d.data_ptr(), m * n, _ptr(sums),
+            _ptr(ws), need, _stream_of(dev)))
+    return (d, sums) if column_sums else d
+
+
 # --------------------------------------------------------------------------- History rows
 def _device_visible(t: Tensor) -> bool:
     return t.is_cuda or t.is_pinned()
@@ -1152,5 +1305,6 @@ def register_torch_ops() -> bool:
 __all__ = [
     "spmm_csr", "spmm_csr_incagg", "rows_sub", "gather_rows", "scatter_rows", "copy_row_chunks",
     "relabel_one_hop", "relabel_one_hop_within_batch", "csr_transpose", "read_async",
-    "write_async", "synchronize", "register_torch_ops",
+    "write_async", "synchronize", "register_torch_ops", "RowGroups", "group_rows",
+    "groups_from_ptr", "grouped_gemm", "grouped_tn",
 ]

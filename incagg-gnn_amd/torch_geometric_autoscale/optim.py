@@ -1,4 +1,6 @@
-"""``Adam`` with the update of ``torch.optim.Adam`` (the optimizer of main.py:160-165) as ONE
+"""``Adam``, gradient norm and clipping.
+
+``Adam`` with the update of ``torch.optim.Adam`` (the optimizer of main.py:160-165) as ONE
 launch over all parameters of a group (incagg_adam_step_f32).
 
 torch's fused multi-tensor kernel walks the tensors in chunks of 65 536 elements: the ~1 M
@@ -7,13 +9,115 @@ advances the step counters); this one gives every 1 024 elements a workgroup.  T
 (one per parameter, as in torch) live on the device and are advanced there, so a step recorded
 into a HIP graph keeps counting when it is replayed.
 """
+import array
 import ctypes
-from typing import Iterable, Union
+from typing import Iterable, List, Optional, Union
 
 import torch
 from torch import Tensor
 
 from . import _lib, ops
+
+NORM_TYPE = {2.0: 2, 1.0: 1, float("inf"): 0}
+
+
+def _norm_type(norm_type) -> int:
+    code = NORM_TYPE.get(float(norm_type))
+    if code is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type}")
+    return code
+
+
+def _max_norm(max_norm) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    return max_norm
+
+
+def _check_grad(g: Tensor, dev) -> None:
+    if not g.is_cuda:
+        raise RuntimeError("gradients must live on the GPU: the norm and clipping kernels are HIP "
+                           "only and there is no CPU implementation")
+    if g.layout != torch.strided or g.dtype not in ops.DTYPE_CODE:
+        raise TypeError(f"gradients must be dense float32, bfloat16 or float16, got {g.dtype}")
+    if g.device != dev:
+        raise ValueError("all gradients must be on one device")
+
+
+def _norm_call(grads: List[Tensor], norm_type: int, max_norm: Optional[float]) -> Tensor:
+    """The norm of contiguous tensors (and their scaling, with ``max_norm``)."""
+    L, dev = _lib.lib(), grads[0].device
+    flat, total = [], 0
+    for g in grads:
+        n = g.numel()
+        total += n
+        flat += (g.data_ptr(), n, ops.DTYPE_CODE[g.dtype])
+    segs = array.array("q", flat)                   # incagg_norm_segment[]
+    need = L.incagg_grad_norm_ws_doubles(len(grads), total)
+    _lib.check(need)
+    ws = torch.empty(max(need, 1), dtype=torch.float64, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    with ops._on_device(dev):
+        if max_norm is None:
+            _lib.check(L.incagg_grad_norm(segs.buffer_info()[0], len(grads), norm_type,
+                                          ws.data_ptr(), need, norm.data_ptr(),
+                                          ops._stream_of(dev)))
+        else:
+            _lib.check(L.incagg_grad_clip(segs.buffer_info()[0], len(grads), norm_type, max_norm,
+                                          ws.data_ptr(), need, norm.data_ptr(),
+                                          ops._stream_of(dev)))
+    return norm
+
+
+def _gradients(parameters) -> List[Tensor]:
+    if isinstance(parameters, Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    for g in grads:
+        _check_grad(g, grads[0].device)
+    return grads
+
+
+@torch.no_grad()
+def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
+    """The norm of all gradients taken as one vector (a float32 scalar on their device;
+    incagg_grad_norm): two launches whatever the number of tensors (up to 128), 64-bit sums in a
+    fixed order.  float32, bfloat16 and float16 gradients may be mixed.  ``norm_type``: 2, 1 or
+    ``inf``."""
+    code = _norm_type(norm_type)
+    grads = _gradients(parameters)
+    if not grads:
+        return torch.zeros(())
+    return _norm_call([g if g.is_contiguous() else g.contiguous() for g in grads], code, None)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
+                    norm_type: float = 2.0, error_if_nonfinite: bool = False) -> Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` (main.py:82-84) in two launches: scales all gradients in
+    place by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm they had
+    (incagg_grad_clip).  Where they need no clipping nothing is written.  Gradients must not
+    overlap in memory.  ``error_if_nonfinite`` waits for the GPU, and raises before anything is
+    scaled.  An optimizer step right behind it can clip as it reads: :meth:`Adam.step`."""
+    code, max_norm = _norm_type(norm_type), _max_norm(max_norm)
+    grads = _gradients(parameters)
+    if not grads:
+        return torch.zeros(())
+    dense = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    if error_if_nonfinite:
+        norm = _norm_call(dense, code, None)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is "
+                               "non-finite, so it cannot be clipped")
+    for g in grads:     # (before anything is scaled)
+        if not g.is_contiguous() and 0 in g.stride() and g.numel() > 1:
+            raise RuntimeError("a gradient's elements overlap in memory (an expanded tensor)")
+    norm = _norm_call(dense, code, max_norm)
+    for g, d in zip(grads, dense):
+        if d is not g:
+            g.copy_(d)
+    return norm
 
 
 class Adam:
@@ -74,7 +178,12 @@ class Adam:
                     p.grad.detach_().zero_()
 
     @torch.no_grad()
-    def step(self) -> None:
+    def step(self, max_norm: Optional[float] = None) -> Optional[Tensor]:
+        """``max_norm``: the gradients are clipped by their global 2-norm (over all groups) as they
+        are read -- ``clip_grad_norm_`` and the step in two launches; ``p.grad`` itself stays as
+        it is -- and the norm they had is returned (a scalar on the device)."""
+        if max_norm is not None:
+            return self._clipped_step(_max_norm(max_norm))
         L = _lib.lib()
         for group in self.param_groups:
             with_grad = [p for p in group["params"] if p.grad is not None]
@@ -98,6 +207,38 @@ class Adam:
                 _lib.check(L.incagg_adam_step_f32(
                     ctypes.addressof(segs), len(with_grad), group["lr"], b1, b2, group["eps"],
                     group["weight_decay"], ops._stream_of(self.device)))
+
+    def _clipped_step(self, max_norm: float) -> Tensor:
+        L, dev = _lib.lib(), self.device
+        flat, keep, total = [], [], 0
+        hyper = (_lib.AdamHyper * len(self.param_groups))()
+        for i, group in enumerate(self.param_groups):
+            b1, b2 = group["betas"]
+            hyper[i] = _lib.AdamHyper(group["lr"], b1, b2, group["eps"], group["weight_decay"])
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.dtype != torch.float32 or g.device != dev:
+                    raise TypeError("gradients must be float32 on the parameter's device")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    keep.append(g)
+                st, n = self.state[p], p.numel()
+                total += n
+                flat += (p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
+                         st["exp_avg_sq"].data_ptr(), st["step"].data_ptr(), n, i)
+        segs = array.array("q", flat)               # incagg_adam_clip_segment[]
+        n_segs = len(flat) // 7
+        need = L.incagg_grad_norm_ws_doubles(n_segs, total)
+        _lib.check(need)
+        ws = torch.empty(max(need, 1), dtype=torch.float64, device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        with ops._on_device(dev):
+            _lib.check(L.incagg_adam_step_clipped_f32(
+                segs.buffer_info()[0], n_segs, ctypes.addressof(hyper), len(hyper), max_norm,
+                ws.data_ptr(), need, norm.data_ptr(), ops._stream_of(dev)))
+        return norm
 
     def state_dict(self) -> dict:
         return {"param_groups": [{k: (v.clone() if isinstance(v, Tensor) else v)

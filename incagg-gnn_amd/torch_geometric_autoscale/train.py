@@ -29,7 +29,7 @@ from .data import gcn_norm, get_data
 from .loader import DeviceSubgraphLoader, EvalSubgraphLoader, SubgraphLoader
 from .metis import load_partition, metis, permute
 from .nn import CrossEntropyLoss
-from .optim import Adam
+from .optim import Adam, clip_grad_norm_
 from .utils import compute_micro_f1, dropout
 
 log = logging.getLogger("incagg.train")
@@ -64,6 +64,12 @@ def mini_train(model, loader, criterion, optimizer, max_steps, grad_norm=None, e
     after its first (eager) execution and replayed whenever the batch comes up again."""
     model.train()
     total_loss, total_examples = 0.0, 0     # the loss sum stays on the device until the end
+    # (the norm is taken over the model's parameters: the optimizer has to hold the same ones)
+    clip_in_step = isinstance(optimizer, Adam) and (
+        {id(p) for g in optimizer.param_groups for p in g["params"]}
+        == {id(p) for p in model.parameters()})
+    clip = (clip_grad_norm_ if torch.device(model.device).type == "cuda"
+            else torch.nn.utils.clip_grad_norm_)
     replayable = (graphs is not None and getattr(loader, "static_batches", False)
                   and not edge_dropout and torch.device(model.device).type == "cuda")
     if replayable:
@@ -101,9 +107,13 @@ def mini_train(model, loader, criterion, optimizer, max_steps, grad_norm=None, e
             optimizer.zero_grad()
             loss = criterion(out.index_select(0, train_idx), y.index_select(0, train_idx))
             loss.backward()
-            if grad_norm is not None:
-                torch.nn.utils.clip_grad_norm_(model.parameters(), grad_norm)
-            optimizer.step()
+            if grad_norm is None:
+                optimizer.step()
+            elif clip_in_step:          # clipped as the optimizer reads them
+                optimizer.step(max_norm=grad_norm)
+            else:
+                clip(model.parameters(), grad_norm)
+                optimizer.step()
             return loss.detach()
 
         if replayable:

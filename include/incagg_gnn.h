@@ -13,7 +13,8 @@
  *     with hipHostMalloc / hipHostRegister, which gfx950 reads over the host link).
  *   - `stream` is a hipStream_t passed as void*; NULL is the default stream.
  *     Kernel entry points only enqueue work; they never synchronise.
- *   - Matrices are fp32, row-major, with a leading dimension given in ELEMENTS.
+ *   - Matrices are fp32 (unless a call takes a dtype), row-major, with a leading dimension
+ *     given in ELEMENTS.
  *   - Device-side CSR uses int32 row pointers and column ids; the int64 forms of
  *     the reference's Python API are converted when a batch is uploaded.
  */
@@ -27,7 +28,7 @@
 extern "C" {
 #endif
 
-#define INCAGG_ABI_VERSION 8
+#define INCAGG_ABI_VERSION 9
 
 enum {
   INCAGG_OK = 0,
@@ -39,6 +40,9 @@ enum {
 };
 
 enum { INCAGG_REDUCE_SUM = 0, INCAGG_REDUCE_MEAN = 1 };
+
+/* Element types of the calls that take one. */
+enum { INCAGG_DTYPE_F32 = 0, INCAGG_DTYPE_BF16 = 1, INCAGG_DTYPE_F16 = 2 };
 
 /* Message of the last failure on the calling thread ("" if none). */
 const char *incagg_last_error(void);
@@ -338,6 +342,87 @@ typedef struct incagg_adam_segment {
 } incagg_adam_segment;
 int incagg_adam_step_f32(const incagg_adam_segment *segs, int64_t n_segs, float lr, float beta1,
                          float beta2, float eps, float weight_decay, void *stream);
+
+/* Global norm of a list of tensors, as torch.nn.utils.clip_grad_norm_ computes it (main.py:82-84):
+ *   *norm = (sum over tensors and elements of |x|^p)^(1/p),  norm_type p = 1 or 2; 0: max |x|
+ * and, in incagg_grad_clip, every element scaled in place by min(1, max_norm / (*norm + 1e-6))
+ * (all of them by 0 where the norm is infinite, to NaN where it is NaN; nothing is read again or
+ * written where the factor is 1).  Sums are held in 64 bits and added in a fixed order.  segs: HOST
+ * array, consumed before the call returns; entries with n == 0 are skipped; tensors may start at
+ * any multiple of their element's size; gradients to be clipped must not overlap.  ws: device
+ * scratch of >= incagg_grad_norm_ws_doubles(n_segs, sum of n); norm: device float.  Launches: one
+ * per 128 tensors to sum, and one more (clip: one per 128) behind them. */
+typedef struct incagg_norm_segment {
+  void *x;
+  int64_t n;
+  int64_t dtype;   /* INCAGG_DTYPE_* */
+} incagg_norm_segment;
+int64_t incagg_grad_norm_ws_doubles(int64_t n_segs, int64_t n_elements);
+int incagg_grad_norm(const incagg_norm_segment *segs, int64_t n_segs, int norm_type, double *ws,
+                     int64_t ws_doubles, float *norm, void *stream);
+int incagg_grad_clip(const incagg_norm_segment *segs, int64_t n_segs, int norm_type,
+                     double max_norm, double *ws, int64_t ws_doubles, float *norm, void *stream);
+
+/* incagg_adam_step_f32 whose gradients are clipped by their global 2-norm as they are read
+ * (main.py:82-85: clip_grad_norm_ and optimizer.step() in two launches): the norm of all g,
+ * g' = g * min(1, max_norm / (norm + 1e-6)) + weight_decay p, and so on.  The gradients themselves
+ * stay as they are; *norm receives the norm.  Every segment names its hyperparameters (an entry of
+ * `hyper`, HOST array) and has a step count of its own; nothing of what is written may overlap.
+ * Bias corrections are evaluated in 64 bits.  ws as for incagg_grad_norm. */
+typedef struct incagg_adam_clip_segment {
+  float *p;
+  const float *g;
+  float *m;
+  float *v;
+  float *step;
+  int64_t n;
+  int64_t hyper;
+} incagg_adam_clip_segment;
+typedef struct incagg_adam_hyper {
+  double lr, beta1, beta2, eps, weight_decay;
+} incagg_adam_hyper;
+int incagg_adam_step_clipped_f32(const incagg_adam_clip_segment *segs, int64_t n_segs,
+                                 const incagg_adam_hyper *hyper, int64_t n_hyper, double max_norm,
+                                 double *ws, int64_t ws_doubles, float *norm, void *stream);
+
+/* ------------------------------------------------------------------ rows of several kinds
+ * Rows ordered by the group (node type, expert, partition) each belongs to: order[rows] holds the
+ * row numbers by ascending ids[i], equal ids in row order, rows of no group (id -1) last;
+ * ptr[g] .. ptr[g + 1] is the range of group g in it, ptr[n_groups] the number of rows that have a
+ * group.  ids: int64 or int32, on the device; an id outside [-1, n_groups) is reported
+ * (incagg_check_device_errors) and its row has no group.  n_groups <=
+ * incagg_group_rows_max_groups(); ws: >= incagg_group_rows_ws_ints(rows, n_groups) device ints.
+ * incagg_group_ptr makes a ptr array of rows that lie sorted already from one of the caller's
+ * (int64 or int32, n_groups + 1 entries): entries that are out of order or outside [0, rows] are
+ * reported and moved to the nearest allowed value. */
+int64_t incagg_group_rows_max_groups(void);
+int64_t incagg_group_rows_ws_ints(int64_t rows, int64_t n_groups);
+int incagg_group_rows(const void *ids, int ids_are_64, int64_t rows, int64_t n_groups, int32_t *ws,
+                      int64_t ws_ints, int32_t *order, int32_t *ptr, void *stream);
+int incagg_group_ptr(const void *in, int in_is_64, int64_t n_groups, int64_t rows, int32_t *out,
+                     void *stream);
+
+/* Products of rows with the weights of their groups, on ptr / order of incagg_group_rows (order
+ * NULL: the rows lie sorted already):
+ *   y[i, :n] = x[i, :k] @ W_g + bias[g, :n]     g the group of row i; W_g = w[g] ([k, n]) or
+ *                                               w[g]^T (w[g]: [n, k], trans_w); bias optional
+ * and y[i] = 0 for rows of no group.  w_group: elements between the weights of two groups.  x, w,
+ * bias and y are of one dtype; sums are held in fp32 and rounded once.  A row number outside
+ * [0, rows) in order is skipped and reported. */
+int incagg_grouped_gemm(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t w_group,
+                        int trans_w, const void *bias, int64_t ld_bias, const int32_t *ptr,
+                        const int32_t *order, int64_t n_groups, int64_t rows, int64_t k, int64_t n,
+                        int dtype, void *y, int64_t ldy, void *stream);
+
+/* The weight gradients of that product: d[g] = sum over the rows i of group g of a[i, :m]^T
+ * b[i, :n] (contiguous [m, n] matrices, d_group elements apart; zeros for a group without rows)
+ * and, when given, sums[g, :m] = the sum of those a[i] (contiguous [n_groups, m]).  Fixed order of
+ * summation.  ws: >= incagg_grouped_tn_ws_bytes(...) bytes on the device. */
+int64_t incagg_grouped_tn_ws_bytes(int64_t n_groups, int64_t rows, int64_t m, int64_t n, int dtype);
+int incagg_grouped_tn(const void *a, int64_t lda, const void *b, int64_t ldb, const int32_t *ptr,
+                      const int32_t *order, int64_t n_groups, int64_t rows, int64_t m, int64_t n,
+                      int dtype, void *d, int64_t d_group, void *sums, void *ws, int64_t ws_bytes,
+                      void *stream);
 
 /* The dense update of a layer on the matrix cores, exact fp32 (v_mfma_f32_32x32x2_f32: a
  * k-ordered chain of fused multiply-adds, one rounding per product):
