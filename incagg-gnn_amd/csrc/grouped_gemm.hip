@@ -17,8 +17,9 @@
 // left out (ml, lm, ll and the two remainders) is below 2^-25 of the product, half a float32
 // rounding, and the sums are float32 as ever.  Six instructions against sixteen.  (A value under
 // 2^-110 keeps an absolute error of 2^-134, bfloat16's smallest step, in place of the relative one.)
-// Infinities, NaNs and values that round to infinity as bfloat16 do not split: the staging code
-// looks for them, and a tile that has one is computed again with plain float32 multiply-adds.
+// Infinities, NaNs and values that round to infinity as bfloat16 do not split: their parts are
+// not finite, so every result they enter is not, and a tile with such a result is computed again
+// with plain float32 multiply-adds.
 //
 // LDS holds K-contiguous tiles, [row][BK], one per part of the split, in 16-byte pieces that are
 // permuted within 128 bytes so that both the fragment reads and the writes spread over the banks.
@@ -89,76 +90,73 @@ template <int BK> __device__ inline int piece_at(int row, int chunk) {
   else return row * 32 + ((chunk ^ (((row >> 1) ^ (row >> 3)) & 3)) << 3);
 }
 
-// Eight values along k of one row: into the parts of its tile (PLANE values apart).
-template <int D, int PLANE>
-__device__ inline void put_piece(unsigned short *tile, int at, const typename Type<D>::Raw (&v)[8],
-                                 unsigned &largest) {
-  if constexpr (D == INCAGG_DTYPE_F32) {
-    u4 h, m, l;
+// Eight float32 values along k of one row: into the three parts of its tile (PLANE values apart).
+template <int PLANE>
+__device__ inline void put_split(unsigned short *tile, int at, const float (&v)[8]) {
+  u4 h, m, l;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      f2 x = {v[2 * i], v[2 * i + 1]};
-      largest = max(largest, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
-      const unsigned hb = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf2));
-      x.x -= __uint_as_float(hb << 16);
-      x.y -= __uint_as_float(hb & 0xffff0000u);
-      const unsigned mb = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf2));
-      x.x -= __uint_as_float(mb << 16);
-      x.y -= __uint_as_float(mb & 0xffff0000u);
-      h[i] = hb;
-      m[i] = mb;
-      l[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf2));
-    }
-    *reinterpret_cast<u4 *>(tile + at) = h;
-    *reinterpret_cast<u4 *>(tile + PLANE + at) = m;
-    *reinterpret_cast<u4 *>(tile + 2 * PLANE + at) = l;
-  } else {
-    u4 h;
-#pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = (unsigned)v[2 * i] | ((unsigned)v[2 * i + 1] << 16);
-    *reinterpret_cast<u4 *>(tile + at) = h;
+  for (int i = 0; i < 4; i++) {
+    f2 x = {v[2 * i], v[2 * i + 1]};
+    const unsigned hb = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf2));
+    x.x -= __uint_as_float(hb << 16);
+    x.y -= __uint_as_float(hb & 0xffff0000u);
+    const unsigned mb = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf2));
+    x.x -= __uint_as_float(mb << 16);
+    x.y -= __uint_as_float(mb & 0xffff0000u);
+    h[i] = hb;
+    m[i] = mb;
+    l[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf2));
   }
+  *reinterpret_cast<u4 *>(tile + at) = h;
+  *reinterpret_cast<u4 *>(tile + PLANE + at) = m;
+  *reinterpret_cast<u4 *>(tile + 2 * PLANE + at) = l;
 }
 
-// A value whose nearest bfloat16 is not finite.
-constexpr unsigned kUnsplittable = 0x7f7f8000u;
-
-// Rows whose k values are contiguous: ROWS x BK, a thread takes U pieces.
+// Rows whose k values are contiguous: ROWS x BK, a thread takes U pieces of 8 values.  The loads
+// of a whole chunk have no condition in them (a branch per piece would make each wait for the one
+// before).
 template <int D, int ROWS, int THREADS> struct RowStage {
   typedef typename Type<D>::Raw Raw;
   static constexpr int BK = Type<D>::BK, CH = BK / 8, UNITS = ROWS * CH;
-  static constexpr int U = (UNITS + THREADS - 1) / THREADS;
+  static constexpr int U = (UNITS + THREADS - 1) / THREADS, W = 2 * sizeof(Raw);
   const Raw *src[U];
-  Pack<Raw, 8> r[U];
+  Pack<unsigned, W> r[U];               // 8 values
+  static __device__ int unit(int i) {
+    const int u = (int)threadIdx.x + i * THREADS;
+    return UNITS % THREADS ? min(u, UNITS - 1) : u;      // (the last piece more than once)
+  }
   template <typename F> __device__ void init(F &&row_of) {
 #pragma unroll
-    for (int i = 0; i < U; i++) {
-      const int u = (int)threadIdx.x + i * THREADS;
-      src[i] = row_of(min(u / CH, ROWS - 1)) + (u % CH) * 8;
-    }
+    for (int i = 0; i < U; i++) src[i] = row_of(unit(i) / CH) + (unit(i) % CH) * 8;
   }
-  __device__ void load(int k0, int k) {
+  __device__ void load(int k0) {
+#pragma unroll
+    for (int i = 0; i < U; i++)
+      r[i] = __builtin_bit_cast(Pack<unsigned, W>,
+                                *reinterpret_cast<const Pack<Raw, 8> *>(src[i] + k0));
+  }
+  __device__ void load_tail(int k0, int k) {
 #pragma unroll
     for (int i = 0; i < U; i++) {
-      const int u = (int)threadIdx.x + i * THREADS, at = k0 + (u % CH) * 8;
-      if (UNITS % THREADS != 0 && u >= UNITS) continue;
-      if (at + 8 <= k) {
-        r[i] = *reinterpret_cast<const Pack<Raw, 8> *>(src[i] + k0);
+      const int left = k - k0 - (unit(i) % CH) * 8;
+      Pack<Raw, 8> v;
+#pragma unroll
+      for (int e = 0; e < 8; e++) v.v[e] = e < left ? src[i][k0 + e] : (Raw)0;
+      r[i] = __builtin_bit_cast(Pack<unsigned, W>, v);
+    }
+  }
+  __device__ void store(unsigned short *tile) {
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      const int at = piece_at<BK>(unit(i) / CH, unit(i) % CH);
+      if constexpr (D == INCAGG_DTYPE_F32) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = __uint_as_float(r[i].v[e]);
+        put_split<ROWS * BK>(tile, at, v);
       } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) r[i].v[e] = at + e < k ? src[i][k0 + e] : (Raw)0;
+        *reinterpret_cast<u4 *>(tile + at) = u4{r[i].v[0], r[i].v[1], r[i].v[2], r[i].v[3]};
       }
-    }
-  }
-  __device__ void store(unsigned short *tile, unsigned &largest) {
-#pragma unroll
-    for (int i = 0; i < U; i++) {
-      const int u = (int)threadIdx.x + i * THREADS;
-      if (UNITS % THREADS != 0 && u >= UNITS) continue;
-      Raw v[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = r[i].v[e];
-      put_piece<D, ROWS * BK>(tile, piece_at<BK>(u / CH, u % CH), v, largest);
     }
   }
 };
@@ -174,29 +172,49 @@ template <int D, int COLS, int THREADS> struct ColStage {
   static __device__ int col() { return ((int)threadIdx.x % GROUPS) * V; }
   static __device__ int row() { return ((int)threadIdx.x / GROUPS) * 8; }
   static __device__ bool active() { return GROUPS * (BK / 8) >= THREADS || row() < BK; }
-  // row i (0 .. 7) of this thread starts at row_of(i), NULL for none; `cols`: columns from this
-  // thread's first one to the matrix's end
-  template <typename F> __device__ void load(int cols, F &&row_of) {
-    if (!active()) return;
+  // row i (0 .. 7) of this thread starts at row_of(i)
+  template <typename F> __device__ void load(F &&row_of) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = *reinterpret_cast<const Pack<Raw, V> *>(row_of(i));
+  }
+  // the same with rows that are not there (NULL); `cols`: columns from this thread's first one to
+  // the matrix's end
+  template <typename F> __device__ void load_tail(int cols, F &&row_of) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const Raw *p = row_of(i);
-      if (p && cols >= V) {
-        r[i] = *reinterpret_cast<const Pack<Raw, V> *>(p);
-      } else {
 #pragma unroll
-        for (int e = 0; e < V; e++) r[i].v[e] = p && e < cols ? p[e] : (Raw)0;
-      }
+      for (int e = 0; e < V; e++) r[i].v[e] = p && e < cols ? p[e] : (Raw)0;
     }
   }
-  __device__ void store(unsigned short *tile, unsigned &largest) {
+  __device__ void clear_row(int i, bool keep) {
+#pragma unroll
+    for (int e = 0; e < V; e++) r[i].v[e] = keep ? r[i].v[e] : (Raw)0;
+  }
+  __device__ void store(unsigned short *tile) {
     if (!active()) return;
 #pragma unroll
     for (int e = 0; e < V; e++) {
-      Raw v[8];
+      const int at = piece_at<BK>(col() + e, row() / 8);
+      if constexpr (D == INCAGG_DTYPE_F32) {
+        float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = r[i].v[e];
-      put_piece<D, COLS * BK>(tile, piece_at<BK>(col() + e, row() / 8), v, largest);
+        for (int i = 0; i < 8; i++) v[i] = r[i].v[e];
+        put_split<COLS * BK>(tile, at, v);
+      } else {
+        u4 h;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if constexpr (V >= 2) {       // halves of two dwords into one
+            const unsigned lo = __builtin_bit_cast(Pack<unsigned, V / 2>, r[2 * i]).v[e / 2];
+            const unsigned hi = __builtin_bit_cast(Pack<unsigned, V / 2>, r[2 * i + 1]).v[e / 2];
+            h[i] = __builtin_amdgcn_perm(hi, lo, e & 1 ? 0x07060302u : 0x05040100u);
+          } else {
+            h[i] = (unsigned)r[2 * i].v[e] | ((unsigned)r[2 * i + 1].v[e] << 16);
+          }
+        }
+        *reinterpret_cast<u4 *>(tile + at) = h;
+      }
     }
   }
 };
@@ -248,6 +266,17 @@ __device__ inline void multiply(const unsigned short *rows, const unsigned short
   }
 }
 
+template <int MI, int NJ> __device__ inline bool all_finite(const f4 (&acc)[MI][NJ]) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < MI; i++)
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s = fmaf(acc[i][j][e], 0.f, s);     // NaN once one is not finite
+  return s == 0.f;
+}
+
 // Four neighbouring results of a row, rounded to their type.
 template <int D> __device__ inline void put_results(void *base, long long at, int count, f4 v) {
   typedef typename Type<D>::Raw Raw;
@@ -267,6 +296,48 @@ template <int D> __device__ inline void put_results(void *base, long long at, in
     for (int e = 0; e < 3; e++)
       if (e < count) p[e] = q.v[e];
   }
+}
+
+// The blocks of a wave as whole rows: each row of 16 blocks goes through LDS (`scratch`, this wave's
+// own, kRowScratch<D, NJ> values), from where a lane stores 16 bytes and neighbouring lanes the next
+// ones.  Straight from the accumulators a store instruction covers 16 rows by 32 or 64 bytes, parts
+// of lines only: 131072 x 2048 bfloat16 results at 1.8 TB/s, 300 us of an 890 us launch.
+// at(row): where the row's first column lies in memory, NULL for a row that is not stored.
+template <int D, int NJ>
+constexpr int kRowScratch = 16 * NJ * 16 * sizeof(typename Type<D>::Raw) / 2;   // (16-bit values)
+
+template <int D, int NJ, typename At>
+__device__ __forceinline__ void put_rows(unsigned short *scratch, const f4 (&v)[NJ], int count,
+                                         At &&at) {
+  typedef typename Type<D>::Raw Raw;
+  constexpr int V = 16 / sizeof(Raw), PIECES = NJ * 16 / V, Q = (16 * PIECES + 63) / 64;
+  static_assert((PIECES & (PIECES - 1)) == 0, "a row is a power of two of pieces");
+  const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+  Raw *rows = reinterpret_cast<Raw *>(scratch);
+#pragma unroll
+  for (int j = 0; j < NJ; j++) {
+    const int col = 16 * j + 4 * quad, place = (col / V) ^ (l16 & (PIECES - 1));
+    put_results<D>(rows, (l16 * PIECES + place) * V + col % V, 4, v[j]);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int q = 0; q < Q; q++) {
+    if (Q * 64 > 16 * PIECES && lane >= 16 * PIECES) continue;
+    const int row = (q * 64 + lane) / PIECES, col = ((lane % PIECES) ^ (row & (PIECES - 1))) * V;
+    const Pack<Raw, V> piece = *reinterpret_cast<const Pack<Raw, V> *>(rows + (q * 64 + lane) * V);
+    Raw *p = at(row);
+    if (!p) continue;
+    if (col + V <= count) {
+      *reinterpret_cast<Pack<Raw, V> *>(p + col) = piece;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V - 1; e++)
+        if (col + e < count) p[col + e] = piece.v[e];
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // ---- finding the work ----------------------------------------------------------------------------
@@ -308,19 +379,62 @@ __device__ inline int row_at(const int *order, int r, int rows, int *err) {
   return -1;
 }
 
+// Results of a wave's blocks, with the bias, into the rows of Y.
+template <int D> struct RowsOut {
+  typedef typename Type<D>::Raw Raw;
+  const GroupedArgs &a;
+  const int g;
+  __device__ f4 bias_at(int n) const {
+    f4 b = {0.f, 0.f, 0.f, 0.f};
+    if (a.bias && g < a.n_groups) {
+      const Raw *p = static_cast<const Raw *>(a.bias) + (long long)g * a.ld_bias + n;
+#pragma unroll
+      for (int e = 0; e < 4; e++) b[e] = n + e < a.n ? raw_to_float<D>(p[e]) : 0.f;
+    }
+    return b;
+  }
+  __device__ void put(int id, int n, f4 v) const {
+    const f4 b = bias_at(n);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] += b[e];
+    put_results<D>(a.y, (long long)id * a.ldy + n, a.n - n, v);
+  }
+  template <int MI, int NJ>
+  __device__ __forceinline__ void put_all(const f4 (&acc)[MI][NJ], const int *ids, int n_first,
+                                          unsigned short *scratch) const {
+    f4 b[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) b[j] = bias_at(n_first + 16 * j + 4 * (((int)threadIdx.x >> 4) & 3));
+#pragma unroll
+    for (int i = 0; i < MI; i++) {
+      f4 v[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[j][e] = acc[i][j][e] + b[j][e];
+      put_rows<D, NJ>(scratch, v, a.n - n_first, [&](int row) -> Raw * {
+        const int id = ids[16 * i + row];
+        return id < 0 ? nullptr : static_cast<Raw *>(a.y) + (long long)id * a.ldy + n_first;
+      });
+    }
+  }
+};
+
 // ---- Y = X W + b -----------------------------------------------------------------------------------
 template <int D, int BM, int BN, int WM, int WN, bool TRANS_W, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN) void grouped_rows_kernel(const GroupedArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_kernel(const GroupedArgs a) {
   typedef typename Type<D>::Raw Raw;
   constexpr int T = 64 * WM * WN, BK = Type<D>::BK, P = Type<D>::P;
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
-  __shared__ __align__(16) unsigned short xt[STAGES][P * BM * BK], wt[STAGES][P * BN * BK];
+  __shared__ __align__(16) unsigned short tiles[STAGES * P * (BM + BN) * BK];
+  unsigned short *const xt = tiles, *const wt = tiles + STAGES * P * BM * BK;
+  static_assert(WM * WN * kRowScratch<D, NJ> <= STAGES * P * (BM + BN) * BK, "space for the results");
   __shared__ int row_ids[BM];
   const int work = xcd_contiguous(blockIdx.x, gridDim.x);
   const int slot = work / a.n_tiles, n0 = (work - slot * a.n_tiles) * BN;
   int g, first, end, tile;
   if (!tile_of_slot<T>(a.ptr, a.n_groups, a.rows, BM, slot, &g, &first, &end, &tile)) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, wave = tid >> 6;
   const int row0 = (wave / WN) * (BM / WM), col0 = (wave % WN) * (BN / WN);
   for (int i = tid; i < BM; i += T)
     row_ids[i] = first + i < end ? row_at(a.order, first + i, a.rows, a.err) : -1;
@@ -337,21 +451,26 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_rows_kernel(const Groupe
     ColStage<D, TRANS_W ? 16 : BN, T> wc;
     if constexpr (TRANS_W) wr.init([&](int c) { return w + (long long)min(n0 + c, a.n - 1) * a.ldw; });
     const int n_chunks = (a.k + BK - 1) / BK;
-    unsigned largest = 0;
+    const bool whole_cols = n0 + BN <= a.n;
     auto load = [&](int c) {
-      xs.load(c * BK, a.k);
+      const int k0 = c * BK;
+      const bool whole = k0 + BK <= a.k;
+      if (whole) xs.load(k0);
+      else xs.load_tail(k0, a.k);
       if constexpr (TRANS_W) {
-        wr.load(c * BK, a.k);
+        if (whole) wr.load(k0);
+        else wr.load_tail(k0, a.k);
       } else {
-        const int r0 = c * BK + wc.row(), n = n0 + wc.col();
+        const int r0 = k0 + wc.row(), n = n0 + wc.col();
         const Raw *p = w + (long long)r0 * a.ldw + n;
-        wc.load(a.n - n, [&](int i) { return r0 + i < a.k ? p + i * a.ldw : nullptr; });
+        if (whole && whole_cols && wc.active()) wc.load([&](int i) { return p + i * a.ldw; });
+        else wc.load_tail(a.n - n, [&](int i) { return r0 + i < a.k ? p + i * a.ldw : nullptr; });
       }
     };
     auto store = [&](int s) {
-      xs.store(xt[s], largest);
-      if constexpr (TRANS_W) wr.store(wt[s], largest);
-      else wc.store(wt[s], largest);
+      xs.store(xt + s * P * BM * BK);
+      if constexpr (TRANS_W) wr.store(wt + s * P * BN * BK);
+      else wc.store(wt + s * P * BN * BK);
     };
     load(0);
     if constexpr (STAGES == 2) {
@@ -359,7 +478,7 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_rows_kernel(const Groupe
       __syncthreads();
       for (int c = 0; c < n_chunks; c++) {
         if (c + 1 < n_chunks) load(c + 1);
-        multiply<D, BM, BN>(xt[c & 1], wt[c & 1], row0, col0, acc);
+        multiply<D, BM, BN>(xt + (c & 1) * P * BM * BK, wt + (c & 1) * P * BN * BK, row0, col0, acc);
         if (c + 1 < n_chunks) store((c + 1) & 1);
         __syncthreads();
       }
@@ -369,49 +488,36 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_rows_kernel(const Groupe
         store(0);
         __syncthreads();
         if (c + 1 < n_chunks) load(c + 1);
-        multiply<D, BM, BN>(xt[0], wt[0], row0, col0, acc);
-      }
-    }
-    if constexpr (D == INCAGG_DTYPE_F32) {
-      if (__syncthreads_or(largest >= kUnsplittable)) {
-        for (int i = 0; i < MI; i++)
-          for (int j = 0; j < NJ; j++)
-            for (int r = 0; r < 4; r++) {
-              const int id = row_ids[row0 + 16 * i + (lane & 15)];
-              const int n = n0 + col0 + 16 * j + 4 * (lane >> 4) + r;
-              float s = 0.f;
-              if (id >= 0 && n < a.n) {
-                const Raw *px = x + (long long)id * a.ldx;
-                const Raw *pw = TRANS_W ? w + (long long)n * a.ldw : w + n;
-                const long long step = TRANS_W ? 1 : a.ldw;
-                for (int k = 0; k < a.k; k++) s = fmaf(px[k], pw[k * step], s);
-              }
-              acc[i][j][r] = s;
-            }
+        multiply<D, BM, BN>(xt, wt, row0, col0, acc);
       }
     }
   }
-
-  const Raw *bias = a.bias && g < a.n_groups
-                        ? static_cast<const Raw *>(a.bias) + (long long)g * a.ld_bias : nullptr;
-#pragma unroll
-  for (int j = 0; j < NJ; j++) {
-    const int n = n0 + col0 + 16 * j + 4 * (lane >> 4);
-    if (n >= a.n) continue;
-    f4 b = {0.f, 0.f, 0.f, 0.f};
-    if (bias)
-#pragma unroll
-      for (int e = 0; e < 4; e++) b[e] = n + e < a.n ? raw_to_float<D>(bias[n + e]) : 0.f;
-#pragma unroll
-    for (int i = 0; i < MI; i++) {
-      const int id = row_ids[row0 + 16 * i + (lane & 15)];
-      if (id < 0) continue;
-      f4 v;
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = acc[i][j][e] + b[e];
-      put_results<D>(a.y, (long long)id * a.ldy + n, a.n - n, v);
+  const RowsOut<D> out{a, g};
+  const int lane = tid & 63;
+  if constexpr (D == INCAGG_DTYPE_F32) {
+    if (g < a.n_groups && __syncthreads_or(!all_finite(acc))) {
+      // (a value that does not split, or a result out of range: plain multiply-adds)
+      for (int ij = 0; ij < MI * NJ; ij++) {
+        const int id = row_ids[row0 + 16 * (ij / NJ) + (lane & 15)];
+        const int n = n0 + col0 + 16 * (ij % NJ) + 4 * (lane >> 4);
+        if (id < 0 || n >= a.n) continue;
+        f4 v;
+        for (int e = 0; e < 4; e++) {
+          const int c = min(n + e, a.n - 1);
+          const Raw *px = x + (long long)id * a.ldx;
+          const Raw *pw = TRANS_W ? w + (long long)c * a.ldw : w + c;
+          const long long step = TRANS_W ? 1 : a.ldw;
+          float s = 0.f;
+          for (int k = 0; k < a.k; k++) s = fmaf(px[k], pw[k * step], s);
+          v[e] = s;
+        }
+        out.put(id, n, v);
+      }
+      return;
     }
   }
+  __syncthreads();                       // (the tiles are read no more)
+  out.put_all(acc, row_ids + row0, n0 + col0, tiles + wave * kRowScratch<D, NJ>);
 }
 
 // ---- D_g = sum A^T B ---------------------------------------------------------------------------------
@@ -423,12 +529,53 @@ __device__ inline long long partial_at(const int *ptr, int g, int rows, int segm
   return 3ll * group_begin(ptr, g, rows) / segment + tile;
 }
 
+// Results of a wave's blocks into D_g, or into the segment's partial.
+template <int D> struct TnOut {
+  const TnArgs &t;
+  const int g, seg;
+  const bool whole;
+  __device__ float *partial() const {
+    const long long part = (long long)t.m * t.n + (t.sums ? t.m : 0);
+    return t.partials + partial_at(t.ptr, g, t.rows, t.segment, seg) * part;
+  }
+  __device__ void put(int m, int n, f4 v) const {
+    const long long e = (long long)m * t.n + n;
+    if (whole) put_results<D>(t.d, g * t.d_group + e, t.n - n, v);
+    else put_results<INCAGG_DTYPE_F32>(partial(), e, t.n - n, v);
+  }
+  __device__ void put_sum(int m, float s) const {
+    const f4 v = {s, 0.f, 0.f, 0.f};
+    if (whole) put_results<D>(t.sums, (long long)g * t.m + m, 1, v);
+    else partial()[(long long)t.m * t.n + m] = s;
+  }
+  template <int MI, int NJ>
+  __device__ __forceinline__ void put_all(const f4 (&acc)[MI][NJ], int m_first, int n_first,
+                                          unsigned short *scratch) const {
+    typedef typename Type<D>::Raw Raw;
+    if (n_first >= t.n) return;
+#pragma unroll
+    for (int i = 0; i < MI; i++) {
+      const int m = m_first + 16 * i;
+      if (whole)
+        put_rows<D, NJ>(scratch, acc[i], t.n - n_first, [&](int row) -> Raw * {
+          return m + row < t.m ? static_cast<Raw *>(t.d) + g * t.d_group + (long long)(m + row) * t.n +
+                                     n_first : nullptr;
+        });
+      else
+        put_rows<INCAGG_DTYPE_F32, NJ>(scratch, acc[i], t.n - n_first, [&](int row) -> float * {
+          return m + row < t.m ? partial() + (long long)(m + row) * t.n + n_first : nullptr;
+        });
+    }
+  }
+};
+
 template <int D, int BM, int BN>
-__global__ __launch_bounds__(256) void grouped_tn_kernel(const TnArgs t) {
+__global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
   typedef typename Type<D>::Raw Raw;
   constexpr int T = 256, BK = Type<D>::BK, P = Type<D>::P;
   constexpr int MI = BM / 32, NJ = BN / 32;
   constexpr int TILES = P * (BM + BN) * BK;
+  static_assert(4 * kRowScratch<INCAGG_DTYPE_F32, NJ> <= TILES, "space for the results");
   __shared__ __align__(16) unsigned short tiles[TILES];
   unsigned short *at = tiles, *bt = tiles + P * BM * BK;
   const int work = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -449,25 +596,67 @@ __global__ __launch_bounds__(256) void grouped_tn_kernel(const TnArgs t) {
   ColStage<D, BM, T> as;
   ColStage<D, BN, T> bs;
   float sums[decltype(as)::V] = {};
-  unsigned largest = 0;
   const int acols = t.m - m0 - as.col(), bcols = t.n - n0 - bs.col();
+  // row numbers of a chunk are fetched one chunk ahead of its rows
+  const bool whole_cols = m0 + BM <= t.m && n0 + BN <= t.n;
+  Pack<int, 8> ia, ib;
+  auto fetch_ids = [&](int r0) {
+    if (!t.order) return;
+    if (r0 + BK <= last) {
+      ia = *reinterpret_cast<const Pack<int, 8> *>(t.order + r0 + min(as.row(), BK - 8));
+      ib = *reinterpret_cast<const Pack<int, 8> *>(t.order + r0 + min(bs.row(), BK - 8));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        ia.v[i] = t.order[min(r0 + as.row() + i, last - 1)];
+        ib.v[i] = t.order[min(r0 + bs.row() + i, last - 1)];
+      }
+    }
+  };
   auto load = [&](int r0) {
+    const Raw *pa = a + m0 + as.col(), *pb = b + n0 + bs.col();
     const int ra = r0 + as.row(), rb = r0 + bs.row();
-    as.load(acols, [&](int i) -> const Raw * {
-      const int id = ra + i < last ? row_at(t.order, ra + i, t.rows, t.err) : -1;
-      return id < 0 ? nullptr : a + (long long)id * t.lda + m0 + as.col();
-    });
-    bs.load(bcols, [&](int i) -> const Raw * {
-      const int id = rb + i < last ? row_at(t.order, rb + i, t.rows, t.err) : -1;
-      return id < 0 ? nullptr : b + (long long)id * t.ldb + n0 + bs.col();
-    });
+    if (r0 + BK <= last && whole_cols && (as.active() && bs.active())) {
+      if (t.order) {
+        as.load([&](int i) { return pa + (long long)min((unsigned)ia.v[i], (unsigned)t.rows - 1u) * t.lda; });
+        bs.load([&](int i) { return pb + (long long)min((unsigned)ib.v[i], (unsigned)t.rows - 1u) * t.ldb; });
+      } else {
+        as.load([&](int i) { return pa + (long long)(ra + i) * t.lda; });
+        bs.load([&](int i) { return pb + (long long)(rb + i) * t.ldb; });
+      }
+    } else {
+      as.load_tail(acols, [&](int i) -> const Raw * {
+        const unsigned id = t.order ? (unsigned)ia.v[i] : (unsigned)(ra + i);
+        return ra + i < last && as.active() ? pa + (long long)min(id, t.rows - 1u) * t.lda : nullptr;
+      });
+      bs.load_tail(bcols, [&](int i) -> const Raw * {
+        const unsigned id = t.order ? (unsigned)ib.v[i] : (unsigned)(rb + i);
+        return rb + i < last && bs.active() ? pb + (long long)min(id, (unsigned)t.rows - 1u) * t.ldb : nullptr;
+      });
+    }
+    if (t.order) {      // rows of no matrix: zeros, and reported
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        bad |= (unsigned)ia.v[i] >= (unsigned)t.rows || (unsigned)ib.v[i] >= (unsigned)t.rows;
+      if (bad) {
+        *t.err = 1;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          as.clear_row(i, (unsigned)ia.v[i] < (unsigned)t.rows);
+          bs.clear_row(i, (unsigned)ib.v[i] < (unsigned)t.rows);
+        }
+      }
+    }
+    if (r0 + BK < last) fetch_ids(r0 + BK);
   };
   if (first < last) {
+    fetch_ids(first);
     load(first);
     for (int r0 = first; r0 < last; r0 += BK) {
       if (r0 > first) __syncthreads();
-      as.store(at, largest);
-      bs.store(bt, largest);
+      as.store(at);
+      bs.store(bt);
       if (want_sums && as.active())
 #pragma unroll
         for (int e = 0; e < decltype(as)::V; e++) {
@@ -481,41 +670,32 @@ __global__ __launch_bounds__(256) void grouped_tn_kernel(const TnArgs t) {
       multiply<D, BM, BN>(at, bt, row0, col0, acc);
     }
   }
-  if constexpr (D == INCAGG_DTYPE_F32) {
-    if (__syncthreads_or(largest >= kUnsplittable)) {
-      for (int i = 0; i < MI; i++)
-        for (int j = 0; j < NJ; j++)
-          for (int e = 0; e < 4; e++) {
-            const int m = m0 + row0 + 16 * i + (lane & 15), n = n0 + col0 + 16 * j + 4 * (lane >> 4) + e;
-            float s = 0.f;
-            if (m < t.m && n < t.n)
-              for (int r = first; r < last; r++) {
-                const int id = row_at(t.order, r, t.rows, t.err);
-                if (id >= 0) s = fmaf(a[(long long)id * t.lda + m], b[(long long)id * t.ldb + n], s);
-              }
-            acc[i][j][e] = s;
-          }
+  const TnOut<D> out{t, g, seg, whole};
+  bool again = false;
+  if constexpr (D == INCAGG_DTYPE_F32) again = __syncthreads_or(!all_finite(acc));
+  if (again) {          // (a value that does not split, or a result out of range)
+    for (int ij = 0; ij < MI * NJ; ij++) {
+      const int m = m0 + row0 + 16 * (ij / NJ) + (lane & 15);
+      const int n = n0 + col0 + 16 * (ij % NJ) + 4 * (lane >> 4);
+      if (m >= t.m || n >= t.n) continue;
+      f4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int r = first; r < last; r++) {
+        const int id = row_at(t.order, r, t.rows, t.err);
+        if (id < 0) continue;
+        const float am = raw_to_float<D>(a[(long long)id * t.lda + m]);
+        const Raw *pb = b + (long long)id * t.ldb;
+        for (int e = 0; e < 4; e++)
+          v[e] = fmaf(am, raw_to_float<D>(pb[min(n + e, t.n - 1)]), v[e]);
+      }
+      out.put(m, n, v);
     }
-  }
-
-  const long long part = (long long)t.m * t.n + (t.sums ? t.m : 0);
-  float *partial = t.partials + partial_at(t.ptr, g, t.rows, t.segment, seg) * part;
-#pragma unroll
-  for (int i = 0; i < MI; i++) {
-    const int m = m0 + row0 + 16 * i + (lane & 15);
-    if (m >= t.m) continue;
-#pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const int n = n0 + col0 + 16 * j + 4 * (lane >> 4);
-      if (n >= t.n) continue;
-      const long long e = (long long)m * t.n + n;
-      if (whole) put_results<D>(t.d, g * t.d_group + e, t.n - n, acc[i][j]);
-      else put_results<INCAGG_DTYPE_F32>(partial, e, t.n - n, acc[i][j]);
-    }
+  } else {
+    __syncthreads();                     // (the tiles are read no more)
+    out.put_all(acc, m0 + row0, n0 + col0, tiles + wave * kRowScratch<INCAGG_DTYPE_F32, NJ>);
   }
   if (!want_sums) return;
   // column sums: threads of one column group, row groups in order
-  constexpr int V = decltype(as)::V, GROUPS = decltype(as)::GROUPS, RG = BK / 8;
+  constexpr int V = decltype(as)::V, RG = BK / 8;
   static_assert(sizeof(float) * RG * BM <= sizeof(tiles), "reduction space");
   float *red = reinterpret_cast<float *>(tiles);
   __syncthreads();
@@ -523,17 +703,339 @@ __global__ __launch_bounds__(256) void grouped_tn_kernel(const TnArgs t) {
 #pragma unroll
     for (int e = 0; e < V; e++) red[(as.row() / 8) * BM + as.col() + e] = sums[e];
   __syncthreads();
-  (void)GROUPS;
   for (int c = tid; c < BM && m0 + c < t.m; c += T) {
     float s = 0.f;
     for (int r = 0; r < RG; r++) s += red[r * BM + c];
-    if (whole) {
-      const f4 v = {s, 0.f, 0.f, 0.f};
-      put_results<D>(t.sums, (long long)g * t.m + m0 + c, 1, v);
-    } else {
-      partial[(long long)t.m * t.n + m0 + c] = s;
+    out.put_sum(m0 + c, s);
+  }
+}
+
+// ---- 16-bit types at full speed: tiles that go from memory into LDS by themselves ----------------------
+// The kernels above pass every tile through registers, which lets them take any alignment and
+// split float32.  For 16-bit operands whose rows are 16-byte aligned the loads write LDS directly
+// (global_load_lds, 16 bytes a lane, 1 KB an instruction, in lane order), without registers or
+// stores.  The LDS image of a chunk (32 values along k) keeps the layout of the matrix:
+//   K-contiguous operand: [row][32 k], 64 bytes a row; piece c of row r lies at c ^ (r / 4 % 4).  A
+//     fragment is one 16-byte read.
+//   K-strided operand: [k][EXT columns]; the 32-byte segment s of row k lies at s ^ f(k), f(k) =
+//     k % 4 + 4 (k / 8 % 2).  A fragment is two transposing reads (ds_read_b64_tr_b16: 16 lanes
+//     name 4 rows x 16 columns, lane i gets column i): the 32 lanes of a read phase touch rows
+//     0..3 and 8..11 of a 16-row block, which f spreads over all 64 banks.
+// The permutation is applied where it is free, to the address each lane loads from (no bank
+// conflicts in either form, by the counters).  What lies past the end of the reduction is loaded
+// from 16 bytes of zeros.
+//
+// Two buffers and one barrier a chunk.  Fragments are read AHEAD row blocks before they are
+// multiplied, so AHEAD blocks before the end of chunk c everything of it is in registers: there the
+// wave waits for the loads of chunk c + 1, meets the others, sends off the loads of c + 2 into the
+// buffer of c and reads the first fragments of c + 1, while the matrix cores work off the last
+// blocks of c.
+constexpr int kDepth = 64;
+__device__ const u4 g_zeros = {0u, 0u, 0u, 0u};
+
+// The instruction has no result register, and its address registers are read when it issues.  (As
+// a builtin, the compiler makes the next LDS read wait for it, whichever buffer that one reads.)
+// m0: where in LDS lane 0's piece goes.
+__device__ inline void load_to_lds(const void *src, unsigned lds_byte) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(lds_byte), "v"(src) : "memory");
+}
+
+// Waits for this wave's loads into LDS; with a barrier behind it, for everybody's.
+__device__ inline void loads_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ inline unsigned lds_byte(const unsigned short *p) {
+  return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) unsigned short *)p;
+}
+
+// Loads of one operand's chunks: wave `wave` of WAVES issues PER instructions for its rows.
+template <bool STRIDED, int EXT, int WAVES> struct LdsTile {
+  static constexpr int PIECES = STRIDED ? EXT / 8 : kDepth / 8;   // 16-byte pieces of an image row
+  static constexpr int ROWS = 64 / PIECES;                        // image rows of an instruction
+  static constexpr int PER = (STRIDED ? kDepth : EXT) / ROWS / WAVES;
+  static constexpr int SIZE = EXT * kDepth;
+  static_assert(PER >= 1 && (PER * ROWS * WAVES == (STRIDED ? kDepth : EXT)), "whole instructions");
+  // image row that this lane loads a piece of, and which piece of the matrix's row goes there
+  static __device__ int row(int wave, int i) {
+    return (wave * PER + i) * ROWS + ((int)threadIdx.x & 63) / PIECES;
+  }
+  static __device__ int piece(int row) {
+    const int at = ((int)threadIdx.x & 63) % PIECES;
+    if constexpr (STRIDED) return at ^ (2 * ((row & 3) | ((row >> 3) & 1) << 2));
+    else return at ^ (row & 7);
+  }
+};
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+__device__ inline s4 read_transposed(const unsigned short *p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s4 *)const_cast<unsigned short *>(p));
+}
+
+// Where this lane's part of a fragment lies: of the fragment at the operand's column (or row) 0.
+template <bool STRIDED, int EXT> __device__ __forceinline__ int fragment_base() {
+  const int l16 = threadIdx.x & 15, quad = (threadIdx.x >> 4) & 3;
+  if constexpr (STRIDED)
+    return (quad * 8 + (l16 >> 2)) * EXT + (((l16 >> 2) | (quad & 1) << 2) << 4) + (l16 & 3) * 4;
+  else
+    return l16 * kDepth + ((quad ^ (l16 & 7)) << 3);
+}
+
+// Fragment of the 16 rows (columns, for a strided operand) from `first` on, k = 32 kk ..
+template <bool STRIDED, int EXT>
+__device__ __forceinline__ u4 fragment(const unsigned short *tile, int base, int first, int kk) {
+  if constexpr (STRIDED) {
+    const unsigned short *p = tile + (base ^ first) + kk * 32 * EXT;    // (segment s ^ f(k))
+    struct { s4 lo, hi; } r = {read_transposed(p), read_transposed(p + 4 * EXT)};
+    return __builtin_bit_cast(u4, r);
+  } else {
+    return *reinterpret_cast<const u4 *>(tile + (base ^ (kk << 5)) + first * kDepth);
+  }
+}
+
+// The pipeline over the chunks of one tile.  load(s): issues the loads of the next chunk, into
+// buffer s.
+template <int D, bool ROWS_STRIDED, bool COLS_STRIDED, int BM, int BN, int WM, int WN>
+struct LdsPipeline {
+  static constexpr int WAVES = WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
+  static constexpr int AHEAD = 2, RING = 4, STEPS = 2 * MI;
+  static_assert(STEPS % RING == 0 && AHEAD < RING && MI >= NJ && NJ % AHEAD == 0, "fragment schedule");
+  typedef LdsTile<ROWS_STRIDED, BM, WAVES> Rows;
+  typedef LdsTile<COLS_STRIDED, BN, WAVES> Cols;
+  static constexpr int CHUNK = Rows::SIZE + Cols::SIZE;         // values of a buffer
+  f4 acc[MI][NJ];
+
+  template <typename Load, typename Extra>
+  __device__ __forceinline__ void run(const unsigned short *tiles, int n_chunks, int row0, int col0,
+                                      Load &&load, Extra &&extra) {
+    u4 a[RING], b[2][NJ];
+    // (the wave's first row goes into the address, the block within the wave is a constant)
+    int ra = fragment_base<ROWS_STRIDED, BM>(), ca = fragment_base<COLS_STRIDED, BN>();
+    ra = ROWS_STRIDED ? ra ^ row0 : ra + row0 * kDepth;
+    ca = COLS_STRIDED ? ca ^ col0 : ca + col0 * kDepth;
+    const auto rows_at = [&](const unsigned short *tile, int i, int kk) __attribute__((always_inline)) {
+      return fragment<ROWS_STRIDED, BM>(tile, ra, 16 * i, kk);
+    };
+    const auto cols_at = [&](const unsigned short *tile, int j, int kk) __attribute__((always_inline)) {
+      return fragment<COLS_STRIDED, BN>(tile + Rows::SIZE, ca, 16 * j, kk);
+    };
+    load(0);
+    loads_landed();
+    __syncthreads();
+    if (n_chunks > 1) load(1);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) b[0][j] = cols_at(tiles, j, 0);
+#pragma unroll
+    for (int t = 0; t < AHEAD; t++) a[t] = rows_at(tiles, t, 0);
+    for (int c = 0; c < n_chunks; c++) {
+      const unsigned short *tile = tiles + (c & 1) * CHUNK, *after = tiles + (~c & 1) * CHUNK;
+      asm volatile("" : "+v"(ra), "+v"(ca));    // (an address per block would not fit the registers)
+#pragma unroll
+      for (int t = 0; t < STEPS; t++) {
+        const int next = t + AHEAD;
+        if (t == STEPS - AHEAD) {       // (behind the last chunk: fragments are read, not used)
+          loads_landed();
+          __syncthreads();
+          if (c + 2 < n_chunks) load(c & 1);
+        }
+        a[next % RING] = next < STEPS ? rows_at(tile, next % MI, next / MI)
+                                      : rows_at(after, next - STEPS, 0);
+        if (t >= MI - NJ && t < MI) b[1][t - (MI - NJ)] = cols_at(tile, t - (MI - NJ), 1);
+        if (t >= STEPS - AHEAD)
+#pragma unroll
+          for (int j = 0; j < NJ / AHEAD; j++)
+            b[0][(t - (STEPS - AHEAD)) * (NJ / AHEAD) + j] =
+                cols_at(after, (t - (STEPS - AHEAD)) * (NJ / AHEAD) + j, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+          acc[t % MI][j] = mfma<D>(b[t / MI][j], a[t % RING], acc[t % MI][j]);
+        extra(t % MI, a[t % RING]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
+};
+
+template <int D, int BM, int BN, int WM, int WN, bool TRANS_W>
+__global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_lds_kernel(const GroupedArgs a) {
+  constexpr int T = 64 * WM * WN;
+  typedef LdsPipeline<D, false, !TRANS_W, BM, BN, WM, WN> Pipe;
+  typedef typename Pipe::Rows X;
+  typedef typename Pipe::Cols W;
+  __shared__ __align__(1024) unsigned short tiles[2 * Pipe::CHUNK];
+  __shared__ int row_ids[BM];
+  const int work = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int slot = work / a.n_tiles, n0 = (work - slot * a.n_tiles) * BN;
+  int g, first, end, tile;
+  if (!tile_of_slot<T>(a.ptr, a.n_groups, a.rows, BM, slot, &g, &first, &end, &tile)) return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row0 = (wave / WN) * (BM / WM), col0 = (wave % WN) * (BN / WN);
+  for (int i = tid; i < BM; i += T)
+    row_ids[i] = first + i < end ? row_at(a.order, first + i, a.rows, a.err) : -1;
+  __syncthreads();
+
+  Pipe pipe{};
+  if (g < a.n_groups) {
+    const unsigned short *x = static_cast<const unsigned short *>(a.x);
+    const unsigned short *w = static_cast<const unsigned short *>(a.w) + (long long)g * a.w_group;
+    // what lies outside the matrices repeats something inside; those results are dropped
+    const unsigned short *px[X::PER], *pw[W::PER];
+    int kx[X::PER], kw[W::PER];         // where along k the lane's piece (or row) is
+#pragma unroll
+    for (int i = 0; i < X::PER; i++) {
+      const int r = X::row(wave, i);
+      kx[i] = X::piece(r) * 8;
+      px[i] = x + (long long)max(row_ids[r], 0) * a.ldx + kx[i];
+    }
+#pragma unroll
+    for (int i = 0; i < W::PER; i++) {
+      const int r = W::row(wave, i);
+      if constexpr (TRANS_W) {
+        kw[i] = W::piece(r) * 8;
+        pw[i] = w + (long long)min(n0 + r, a.n - 1) * a.ldw + kw[i];
+      } else {
+        kw[i] = r;
+        pw[i] = w + (long long)r * a.ldw + min(n0 + W::piece(r) * 8, a.n - 8);
+      }
+    }
+    const long long w_step = TRANS_W ? kDepth : kDepth * a.ldw;
+    const unsigned base = __builtin_amdgcn_readfirstlane(lds_byte(tiles));
+    int left = a.k;                     // of the reduction, from the next chunk on
+    auto load = [&](int s) __attribute__((always_inline)) {
+      const unsigned to = base + s * Pipe::CHUNK * 2 + wave * X::PER * 1024;
+      const unsigned wo = base + s * Pipe::CHUNK * 2 + X::SIZE * 2 + wave * W::PER * 1024;
+      if (left >= kDepth) {
+#pragma unroll
+        for (int i = 0; i < X::PER; i++) load_to_lds(px[i], to + i * 1024);
+#pragma unroll
+        for (int i = 0; i < W::PER; i++) load_to_lds(pw[i], wo + i * 1024);
+      } else {
+#pragma unroll
+        for (int i = 0; i < X::PER; i++)
+          load_to_lds(kx[i] < left ? (const void *)px[i] : (const void *)&g_zeros, to + i * 1024);
+#pragma unroll
+        for (int i = 0; i < W::PER; i++)
+          load_to_lds(kw[i] < left ? (const void *)pw[i] : (const void *)&g_zeros, wo + i * 1024);
+      }
+#pragma unroll
+      for (int i = 0; i < X::PER; i++) px[i] += kDepth;
+#pragma unroll
+      for (int i = 0; i < W::PER; i++) pw[i] += w_step;
+      left -= kDepth;
+    };
+    pipe.run(tiles, (a.k + kDepth - 1) / kDepth, row0, col0, load, [](int, u4) {});
+  }
+  const RowsOut<D> out{a, g};
+  __syncthreads();                       // (the tiles are read no more)
+  out.put_all(pipe.acc, row_ids + row0, n0 + col0, tiles + wave * kRowScratch<D, Pipe::NJ>);
+}
+
+// D_g over one segment; the column sums of A come from the matrix cores too, as one more column
+// block of ones (exact products, the same float32 sums).  Row numbers come through the scalar
+// cache: a vector load of them would have to be waited for, and with it all tile loads behind it.
+template <int D, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void grouped_tn_lds_kernel(const TnArgs t) {
+  constexpr int T = 64 * WM * WN;
+  typedef LdsPipeline<D, true, true, BM, BN, WM, WN> Pipe;
+  typedef typename Pipe::Rows A;
+  typedef typename Pipe::Cols B;
+  static_assert(A::PER * A::ROWS == B::PER * B::ROWS, "a wave loads the same rows of both");
+  constexpr int WAVE_ROWS = A::PER * A::ROWS;
+  __shared__ __align__(1024) unsigned short tiles[2 * Pipe::CHUNK];
+  const int work = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int per_slot = t.m_tiles * t.n_tiles, slot = work / per_slot, mn = work - slot * per_slot;
+  const int m0 = (mn / t.n_tiles) * BM, n0 = (mn % t.n_tiles) * BN;
+  int g, first, end, seg;
+  const bool any = tile_of_slot<T>(t.ptr, t.n_groups, t.rows, t.segment, slot, &g, &first, &end, &seg);
+  if (g >= t.n_groups || seg < 0 || (!any && seg > 0)) return;
+  g = __builtin_amdgcn_readfirstlane(g);
+  const int begin = group_begin(t.ptr, g, t.rows);
+  const bool whole = end - begin <= t.segment;       // the group's only segment (or an empty group)
+  const int last = __builtin_amdgcn_readfirstlane(min(end, first + t.segment));
+  first = __builtin_amdgcn_readfirstlane(first);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row0 = (wave / WN) * (BM / WM), col0 = (wave % WN) * (BN / WN);
+  const bool want_sums = t.sums && n0 == 0 && col0 == 0;
+
+  // the columns each lane's pieces begin at (instructions i and i + 2: the same piece)
+  constexpr int CA = A::PER < 2 ? A::PER : 2, CB = B::PER < 2 ? B::PER : 2;
+  int ca[CA], cb[CB];
+#pragma unroll
+  for (int i = 0; i < CA; i++) ca[i] = min(m0 + A::piece(A::row(wave, i)) * 8, t.m - 8);
+#pragma unroll
+  for (int i = 0; i < CB; i++) cb[i] = min(n0 + B::piece(B::row(wave, i)) * 8, t.n - 8);
+  const auto *order = (const __attribute__((address_space(4))) int *)t.order;
+  int ids[WAVE_ROWS];                   // row numbers of the next chunk to load (-1: zeros)
+  int bad = 0;
+  int next_row = first + wave * WAVE_ROWS;
+  auto fetch_ids = [&]() __attribute__((always_inline)) {
+    if (order) {
+#pragma unroll
+      for (int i = 0; i < WAVE_ROWS; i++)
+        ids[i] = __builtin_amdgcn_readfirstlane(order[min(next_row + i, last - 1)]);
+#pragma unroll
+      for (int i = 0; i < WAVE_ROWS; i++) {
+        const int outside = (unsigned)ids[i] >= (unsigned)t.rows;
+        bad |= outside;
+        ids[i] = next_row + i < last && !outside ? ids[i] : -1;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < WAVE_ROWS; i++) ids[i] = next_row + i < last ? next_row + i : -1;
+    }
+    next_row += kDepth;
+  };
+  const unsigned base = __builtin_amdgcn_readfirstlane(lds_byte(tiles));
+  const int n_chunks = (last - first + kDepth - 1) / kDepth;
+  auto load = [&](int s) __attribute__((always_inline)) {
+    const unsigned ao = base + s * Pipe::CHUNK * 2 + wave * A::PER * 1024;
+    const unsigned bo = base + s * Pipe::CHUNK * 2 + A::SIZE * 2 + wave * B::PER * 1024;
+    // row `of` (of this lane) among the wave's rows
+    auto id_of = [&](int i, int rows, int of) __attribute__((always_inline)) {
+      int id = ids[i * rows];
+#pragma unroll
+      for (int j = 1; j < rows; j++) id = of == j ? ids[i * rows + j] : id;
+      return id;
+    };
+#pragma unroll
+    for (int i = 0; i < A::PER; i++) {
+      const int id = id_of(i, A::ROWS, lane / A::PIECES);
+      const unsigned short *p = static_cast<const unsigned short *>(t.a) + id * t.lda + ca[i % CA];
+      load_to_lds(id < 0 ? (const void *)&g_zeros : (const void *)p, ao + i * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < B::PER; i++) {
+      const int id = id_of(i, B::ROWS, lane / B::PIECES);
+      const unsigned short *p = static_cast<const unsigned short *>(t.b) + id * t.ldb + cb[i % CB];
+      load_to_lds(id < 0 ? (const void *)&g_zeros : (const void *)p, bo + i * 1024);
+    }
+    fetch_ids();                        // (behind the last chunk: zeros)
+  };
+
+  Pipe pipe{};
+  f4 sums[Pipe::MI] = {};
+  const u4 ones = D == INCAGG_DTYPE_BF16 ? u4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
+                                         : u4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+  if (first < last) {
+    fetch_ids();
+    if (want_sums)
+      pipe.run(tiles, n_chunks, row0, col0, load,
+               [&](int i, u4 a) __attribute__((always_inline)) { sums[i] = mfma<D>(ones, a, sums[i]); });
+    else
+      pipe.run(tiles, n_chunks, row0, col0, load, [](int, u4) {});
+    if (bad) *t.err = 1;
+  }
+  const TnOut<D> out{t, g, seg, whole};
+  __syncthreads();                       // (the tiles are read no more)
+  out.put_all(pipe.acc, m0 + row0, n0 + col0,
+              tiles + wave * kRowScratch<INCAGG_DTYPE_F32, Pipe::NJ>);
+  if (want_sums && lane < 16)
+#pragma unroll
+    for (int i = 0; i < Pipe::MI; i++) {
+      const int m = m0 + row0 + 16 * i + lane;
+      if (m < t.m) out.put_sum(m, sums[i][0]);
+    }
 }
 
 template <int D> __global__ __launch_bounds__(256) void grouped_tn_finish_kernel(const TnArgs t) {
@@ -582,7 +1084,37 @@ static int launch_rows_tile(GroupedArgs &a, bool trans_w, hipStream_t s) {
   return INCAGG_OK;
 }
 
+template <int D, int BM, int BN, int WM, int WN>
+static int launch_rows_lds(GroupedArgs &a, bool trans_w, hipStream_t s) {
+  a.n_tiles = (a.n + BN - 1) / BN;
+  const int64_t blocks = ((int64_t)a.rows / BM + a.n_groups + 1) * a.n_tiles;
+  INCAGG_REQUIRE(blocks < (1ll << 31), "too many rows and columns for one call");
+  const dim3 grid((unsigned)blocks), block(64 * WM * WN);
+  if (trans_w)
+    hipLaunchKernelGGL((grouped_rows_lds_kernel<D, BM, BN, WM, WN, true>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((grouped_rows_lds_kernel<D, BM, BN, WM, WN, false>), grid, block, 0, s, a);
+  INCAGG_HIP_TRY(hipGetLastError());
+  return INCAGG_OK;
+}
+
+// Rows in whole 16-byte pieces.
+static bool pieces(const void *p, int64_t ld, int64_t width) {
+  return aligned16(p) && ld % 8 == 0 && width % 8 == 0;
+}
+
 template <int D> static int launch_rows(GroupedArgs &a, bool trans_w, hipStream_t s) {
+  if constexpr (D != INCAGG_DTYPE_F32) {
+    if ((int64_t)a.rows > 48ll * a.n_groups && a.n > 64 && pieces(a.x, a.ldx, a.k) &&
+        pieces(a.w, a.ldw, trans_w ? a.k : a.n) && a.w_group % 8 == 0) {
+      // 256 x 256 halves what a tile reads for its products, but leaves one workgroup to a CU: for
+      // at least one round of them (128 x 128 against it, 131072 x 1024 -> 2048: 848 / 671 us,
+      // 32768 x 1024 -> 1024, two rounds: 93 / 90 us)
+      const int64_t tiles = ((int64_t)a.rows / 256 + a.n_groups / 2) * ((a.n + 255) / 256);
+      if (a.n <= 128 || tiles < 256) return launch_rows_lds<D, 128, 128, 2, 2>(a, trans_w, s);
+      return launch_rows_lds<D, 256, 256, 2, 4>(a, trans_w, s);
+    }
+  }
   constexpr int STAGES = D == INCAGG_DTYPE_F32 ? 1 : 2;
   // few rows to a group: the weights are what is read, and a tall tile would be mostly empty
   if ((int64_t)a.rows <= 48ll * a.n_groups)
@@ -599,6 +1131,16 @@ static int tn_segment(int64_t rows, int64_t m, int64_t n) {
   return (int)((s + 63) / 64 * 64);
 }
 
+// Adds up the partials of groups that were cut into segments.
+template <int D> static int tn_finish(TnArgs &t, hipStream_t s) {
+  if (t.rows <= t.segment) return INCAGG_OK;
+  const int64_t part = (int64_t)t.m * t.n + (t.sums ? t.m : 0);
+  hipLaunchKernelGGL(grouped_tn_finish_kernel<D>,
+                     dim3((unsigned)((part + 1023) / 1024), (unsigned)t.n_groups), dim3(256), 0, s, t);
+  INCAGG_HIP_TRY(hipGetLastError());
+  return INCAGG_OK;
+}
+
 template <int D, int BM, int BN> static int launch_tn_tile(TnArgs &t, hipStream_t s) {
   t.m_tiles = (t.m + BM - 1) / BM;
   t.n_tiles = (t.n + BN - 1) / BN;
@@ -606,16 +1148,26 @@ template <int D, int BM, int BN> static int launch_tn_tile(TnArgs &t, hipStream_
   INCAGG_REQUIRE(blocks < (1ll << 31), "too many rows and columns for one call");
   hipLaunchKernelGGL((grouped_tn_kernel<D, BM, BN>), dim3((unsigned)blocks), dim3(256), 0, s, t);
   INCAGG_HIP_TRY(hipGetLastError());
-  if (t.rows > t.segment) {
-    const int64_t part = (int64_t)t.m * t.n + (t.sums ? t.m : 0);
-    hipLaunchKernelGGL(grouped_tn_finish_kernel<D>,
-                       dim3((unsigned)((part + 1023) / 1024), (unsigned)t.n_groups), dim3(256), 0, s, t);
-    INCAGG_HIP_TRY(hipGetLastError());
-  }
-  return INCAGG_OK;
+  return tn_finish<D>(t, s);
+}
+
+template <int D, int BM, int BN, int WM, int WN>
+static int launch_tn_lds(TnArgs &t, hipStream_t s) {
+  t.m_tiles = (t.m + BM - 1) / BM;
+  t.n_tiles = (t.n + BN - 1) / BN;
+  const int64_t blocks = ((int64_t)t.rows / t.segment + t.n_groups) * t.m_tiles * t.n_tiles;
+  INCAGG_REQUIRE(blocks < (1ll << 31), "too many rows and columns for one call");
+  hipLaunchKernelGGL((grouped_tn_lds_kernel<D, BM, BN, WM, WN>), dim3((unsigned)blocks),
+                     dim3(64 * WM * WN), 0, s, t);
+  INCAGG_HIP_TRY(hipGetLastError());
+  return tn_finish<D>(t, s);
 }
 
 template <int D> static int launch_tn(TnArgs &t, hipStream_t s) {
+  if constexpr (D != INCAGG_DTYPE_F32) {
+    if (t.m > 128 && t.n > 128 && pieces(t.a, t.lda, t.m) && pieces(t.b, t.ldb, t.n))
+      return launch_tn_lds<D, 256, 256, 2, 4>(t, s);
+  }
   if (t.m <= 64) return t.n <= 64 ? launch_tn_tile<D, 64, 64>(t, s) : launch_tn_tile<D, 64, 128>(t, s);
   return t.n <= 64 ? launch_tn_tile<D, 128, 64>(t, s) : launch_tn_tile<D, 128, 128>(t, s);
 }
