@@ -139,9 +139,20 @@ template <int D, int ROWS, int THREADS> struct RowStage {
 #pragma unroll
     for (int i = 0; i < U; i++) {
       const int left = k - k0 - (unit(i) % CH) * 8;
+      constexpr int N = 16 / sizeof(Raw);
       Pack<Raw, 8> v;
 #pragma unroll
-      for (int e = 0; e < 8; e++) v.v[e] = e < left ? src[i][k0 + e] : (Raw)0;
+      for (int h = 0; h < 8; h += N) {
+        Pack<Raw, N> q;
+        if (left >= h + N) {
+          q = *reinterpret_cast<const Pack<Raw, N> *>(src[i] + k0 + h);
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; e++) q.v[e] = h + e < left ? src[i][k0 + h + e] : (Raw)0;
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) v.v[h + e] = q.v[e];
+      }
       r[i] = __builtin_bit_cast(Pack<unsigned, W>, v);
     }
   }
@@ -183,10 +194,18 @@ template <int D, int COLS, int THREADS> struct ColStage {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const Raw *p = row_of(i);
+      if (p && cols >= V) {
+        r[i] = *reinterpret_cast<const Pack<Raw, V> *>(p);
+      } else {
 #pragma unroll
-      for (int e = 0; e < V; e++) r[i].v[e] = p && e < cols ? p[e] : (Raw)0;
+        for (int e = 0; e < V; e++) r[i].v[e] = p && e < cols ? p[e] : (Raw)0;
+      }
     }
   }
+  // The thread's first column, of a matrix of n, when its columns end where vectors do: columns
+  // behind the last repeat the last vector (their results are dropped).
+  static __device__ bool whole_vectors(int first, int n) { return first + COLS <= n || (n >= V && n % V == 0); }
+  static __device__ int col_within(int first, int n) { return first + COLS <= n ? first + col() : min(first + col(), n - V); }
   __device__ void clear_row(int i, bool keep) {
 #pragma unroll
     for (int e = 0; e < V; e++) r[i].v[e] = keep ? r[i].v[e] : (Raw)0;
@@ -451,8 +470,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_kernel(const Gro
     ColStage<D, TRANS_W ? 16 : BN, T> wc;
     if constexpr (TRANS_W) wr.init([&](int c) { return w + (long long)min(n0 + c, a.n - 1) * a.ldw; });
     const int n_chunks = (a.k + BK - 1) / BK;
-    const bool whole_cols = n0 + BN <= a.n;
-    auto load = [&](int c) {
+    const bool whole_cols = wc.whole_vectors(n0, a.n);
+    auto load = [&](int c) __attribute__((always_inline)) {
       const int k0 = c * BK;
       const bool whole = k0 + BK <= a.k;
       if (whole) xs.load(k0);
@@ -461,13 +480,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_kernel(const Gro
         if (whole) wr.load(k0);
         else wr.load_tail(k0, a.k);
       } else {
-        const int r0 = k0 + wc.row(), n = n0 + wc.col();
+        const int r0 = k0 + wc.row(), n = whole_cols ? wc.col_within(n0, a.n) : n0 + wc.col();
         const Raw *p = w + (long long)r0 * a.ldw + n;
-        if (whole && whole_cols && wc.active()) wc.load([&](int i) { return p + i * a.ldw; });
-        else wc.load_tail(a.n - n, [&](int i) { return r0 + i < a.k ? p + i * a.ldw : nullptr; });
+        if (whole && whole_cols && wc.active())
+          wc.load([&](int i) { return p + i * a.ldw; });
+        else
+          wc.load_tail(a.n - n, [&](int i) { return r0 + i < a.k ? p + i * a.ldw : nullptr; });
       }
     };
-    auto store = [&](int s) {
+    auto store = [&](int s) __attribute__((always_inline)) {
       xs.store(xt + s * P * BM * BK);
       if constexpr (TRANS_W) wr.store(wt + s * P * BN * BK);
       else wc.store(wt + s * P * BN * BK);
@@ -598,7 +619,9 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
   float sums[decltype(as)::V] = {};
   const int acols = t.m - m0 - as.col(), bcols = t.n - n0 - bs.col();
   // row numbers of a chunk are fetched one chunk ahead of its rows
-  const bool whole_cols = m0 + BM <= t.m && n0 + BN <= t.n;
+  const bool whole_a = as.whole_vectors(m0, t.m), whole_b = bs.whole_vectors(n0, t.n);
+  const Raw *const pa = a + (whole_a ? as.col_within(m0, t.m) : m0 + as.col());
+  const Raw *const pb = b + (whole_b ? bs.col_within(n0, t.n) : n0 + bs.col());
   Pack<int, 8> ia, ib;
   auto fetch_ids = [&](int r0) {
     if (!t.order) return;
@@ -614,26 +637,25 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
     }
   };
   auto load = [&](int r0) {
-    const Raw *pa = a + m0 + as.col(), *pb = b + n0 + bs.col();
     const int ra = r0 + as.row(), rb = r0 + bs.row();
-    if (r0 + BK <= last && whole_cols && (as.active() && bs.active())) {
-      if (t.order) {
-        as.load([&](int i) { return pa + (long long)min((unsigned)ia.v[i], (unsigned)t.rows - 1u) * t.lda; });
-        bs.load([&](int i) { return pb + (long long)min((unsigned)ib.v[i], (unsigned)t.rows - 1u) * t.ldb; });
-      } else {
-        as.load([&](int i) { return pa + (long long)(ra + i) * t.lda; });
-        bs.load([&](int i) { return pb + (long long)(rb + i) * t.ldb; });
-      }
-    } else {
-      as.load_tail(acols, [&](int i) -> const Raw * {
-        const unsigned id = t.order ? (unsigned)ia.v[i] : (unsigned)(ra + i);
-        return ra + i < last && as.active() ? pa + (long long)min(id, t.rows - 1u) * t.lda : nullptr;
+    // (only rows inside the matrices are named)
+    auto row_a = [&](int i) {
+      return pa + (long long)(t.order ? min((unsigned)ia.v[i], (unsigned)t.rows - 1u) : ra + i) * t.lda;
+    };
+    auto row_b = [&](int i) {
+      return pb + (long long)(t.order ? min((unsigned)ib.v[i], (unsigned)t.rows - 1u) : rb + i) * t.ldb;
+    };
+    const bool whole_rows = r0 + BK <= last;
+    if (whole_rows && whole_a && as.active()) as.load(row_a);
+    else
+      as.load_tail(whole_a ? BM : acols, [&](int i) -> const Raw * {
+        return ra + i < last && as.active() ? row_a(i) : nullptr;
       });
-      bs.load_tail(bcols, [&](int i) -> const Raw * {
-        const unsigned id = t.order ? (unsigned)ib.v[i] : (unsigned)(rb + i);
-        return rb + i < last && bs.active() ? pb + (long long)min(id, (unsigned)t.rows - 1u) * t.ldb : nullptr;
+    if (whole_rows && whole_b && bs.active()) bs.load(row_b);
+    else
+      bs.load_tail(whole_b ? BN : bcols, [&](int i) -> const Raw * {
+        return rb + i < last && bs.active() ? row_b(i) : nullptr;
       });
-    }
     if (t.order) {      // rows of no matrix: zeros, and reported
       bool bad = false;
 #pragma unroll
@@ -1038,34 +1060,47 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_tn_lds_kernel(const T
     }
 }
 
+// Partials of groups that were cut into segments, added up: 32 x 4 neighbouring elements to a
+// workgroup, every eighth segment to a thread (in order), the eight sums in order.
 template <int D> __global__ __launch_bounds__(256) void grouped_tn_finish_kernel(const TnArgs t) {
+  __shared__ f4 sums[8][32];
   const int g = blockIdx.y;
   const int begin = group_begin(t.ptr, g, t.rows), end = group_begin(t.ptr, g + 1, t.rows);
   if (end - begin <= t.segment) return;
   const int segments = (end - begin + t.segment - 1) / t.segment;
   const long long mn = (long long)t.m * t.n, part = mn + (t.sums ? t.m : 0);
-  const long long e = (blockIdx.x * 256ll + threadIdx.x) * 4;
-  if (e >= part) return;
-  const float *p = t.partials + partial_at(t.ptr, g, t.rows, t.segment, 0) * part + e;
-  const int count = (int)min(4ll, part - e);
-  f4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < segments; i++, p += part) {
-    if (count == 4) {
-      const Pack<float, 4> q = *reinterpret_cast<const Pack<float, 4> *>(p);
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  for (long long first = blockIdx.x * 128ll; first < part; first += gridDim.x * 128ll) {
+    const long long e = first + lane * 4;
+    const float *p = t.partials + partial_at(t.ptr, g, t.rows, t.segment, row) * part + e;
+    const int count = (int)max(0ll, min(4ll, part - e));
+    f4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = row; i < segments; i += 8, p += 8 * part) {
+      if (count == 4) {
+        const Pack<float, 4> q = *reinterpret_cast<const Pack<float, 4> *>(p);
 #pragma unroll
-      for (int j = 0; j < 4; j++) s[j] += q.v[j];
-    } else {
-      for (int j = 0; j < count; j++) s[j] += p[j];
+        for (int j = 0; j < 4; j++) s[j] += q.v[j];
+      } else {
+        for (int j = 0; j < count; j++) s[j] += p[j];
+      }
     }
-  }
-  if (e + 4 <= mn) {
-    put_results<D>(t.d, g * t.d_group + e, 4, s);
-  } else {
-    for (int j = 0; j < count; j++) {
-      const f4 v = {s[j], 0.f, 0.f, 0.f};
-      if (e + j < mn) put_results<D>(t.d, g * t.d_group + e + j, 1, v);
-      else put_results<D>(t.sums, (long long)g * t.m + (e + j - mn), 1, v);
+    sums[row][lane] = s;
+    __syncthreads();
+    if (row == 0 && count > 0) {
+#pragma unroll
+      for (int i = 1; i < 8; i++) s += sums[i][lane];
+      if (e + 4 <= mn) {
+        put_results<D>(t.d, g * t.d_group + e, 4, s);
+      } else {
+        for (int j = 0; j < count; j++) {
+          const f4 v = {s[j], 0.f, 0.f, 0.f};
+          if (e + j < mn) put_results<D>(t.d, g * t.d_group + e + j, 1, v);
+          else put_results<D>(t.sums, (long long)g * t.m + (e + j - mn), 1, v);
+        }
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -1123,11 +1158,19 @@ template <int D> static int launch_rows(GroupedArgs &a, bool trans_w, hipStream_
   return launch_rows_tile<D, 128, 128, 2, 2, STAGES>(a, trans_w, s);
 }
 
-// Rows of a segment: enough segments to fill the chip (about 1024 workgroups), at least 512 rows.
-static int tn_segment(int64_t rows, int64_t m, int64_t n) {
-  const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128);
-  const int64_t wanted = std::max<int64_t>(1, 1024 / tiles);
-  const int64_t s = std::max<int64_t>(512, (rows + wanted - 1) / wanted);
+// Whether the weight gradient runs in 256 x 256 tiles where the operands' alignment allows it.
+static bool tn_large_tiles(int64_t m, int64_t n, int dtype) {
+  return dtype != INCAGG_DTYPE_F32 && m > 128 && n > 128;
+}
+
+// Rows of a segment: enough segments to fill the chip (one workgroup to a CU of 256 x 256 tiles,
+// two of 128 x 128), at least 256 rows.  Shorter ones even out groups of different sizes, but every
+// one of a longer group costs a partial written and read.
+static int tn_segment(int64_t rows, int64_t m, int64_t n, int dtype) {
+  const bool large = tn_large_tiles(m, n, dtype);
+  const int64_t tile = large ? 256 : 128, tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
+  const int64_t wanted = std::max<int64_t>(1, (large ? 256 : 512) / tiles);
+  const int64_t s = std::max<int64_t>(256, (rows + wanted - 1) / wanted);
   return (int)((s + 63) / 64 * 64);
 }
 
@@ -1136,7 +1179,8 @@ template <int D> static int tn_finish(TnArgs &t, hipStream_t s) {
   if (t.rows <= t.segment) return INCAGG_OK;
   const int64_t part = (int64_t)t.m * t.n + (t.sums ? t.m : 0);
   hipLaunchKernelGGL(grouped_tn_finish_kernel<D>,
-                     dim3((unsigned)((part + 1023) / 1024), (unsigned)t.n_groups), dim3(256), 0, s, t);
+                     dim3((unsigned)std::min<int64_t>((part + 127) / 128, 512), (unsigned)t.n_groups),
+                     dim3(256), 0, s, t);
   INCAGG_HIP_TRY(hipGetLastError());
   return INCAGG_OK;
 }
@@ -1165,7 +1209,7 @@ static int launch_tn_lds(TnArgs &t, hipStream_t s) {
 
 template <int D> static int launch_tn(TnArgs &t, hipStream_t s) {
   if constexpr (D != INCAGG_DTYPE_F32) {
-    if (t.m > 128 && t.n > 128 && pieces(t.a, t.lda, t.m) && pieces(t.b, t.ldb, t.n))
+    if (tn_large_tiles(t.m, t.n, D) && pieces(t.a, t.lda, t.m) && pieces(t.b, t.ldb, t.n))
       return launch_tn_lds<D, 256, 256, 2, 4>(t, s);
   }
   if (t.m <= 64) return t.n <= 64 ? launch_tn_tile<D, 64, 64>(t, s) : launch_tn_tile<D, 64, 128>(t, s);
@@ -1219,7 +1263,7 @@ extern "C" int64_t incagg_grouped_tn_ws_bytes(int64_t n_groups, int64_t rows, in
   if (n_groups < 1 || rows < 0 || rows > INT_MAX - 4096 || m < 1 || n < 1 || m >= (1 << 20) ||
       n >= (1 << 20))
     return fail(INCAGG_E_INVALID, "size out of range");
-  const int64_t segment = tn_segment(rows, m, n);
+  const int64_t segment = tn_segment(rows, m, n, dtype);
   return rows <= segment ? 0 : (3 * rows / segment + 1) * (m * n + m) * (int64_t)sizeof(float);
 }
 
@@ -1241,7 +1285,7 @@ extern "C" int incagg_grouped_tn(const void *a, int64_t lda, const void *b, int6
                  (long long)ws_bytes, (long long)need);
   TnArgs t{};
   t.partials = static_cast<float *>(ws);
-  t.segment = tn_segment(rows, m, n);
+  t.segment = tn_segment(rows, m, n, dtype);
   t.a = a; t.b = b; t.d = d; t.sums = sums; t.lda = lda; t.ldb = ldb; t.d_group = d_group;
   t.ptr = ptr; t.order = order; t.n_groups = (int)n_groups; t.rows = (int)rows;
   t.m = (int)m; t.n = (int)n;
