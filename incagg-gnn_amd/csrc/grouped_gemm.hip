@@ -365,21 +365,34 @@ __device__ inline int group_begin(const int *ptr, int g, int rows) {
   return g == 0 ? 0 : min(max(ptr[g], 0), rows);
 }
 
-// The row tile of a slot: false if the slot is empty.  g == n_groups: rows of no group.
+// The row tile of a slot: false if the slot is empty.  g == n_groups: rows of no group.  The
+// thread that holds a bound hands it on through LDS: reading ptr again would put another memory
+// latency in front of every tile.
 template <int THREADS>
 __device__ inline bool tile_of_slot(const int *ptr, int n_groups, int rows, int tile_rows, int slot,
                                     int *g, int *first, int *end, int *tile) {
-  int before = 0;
+  __shared__ int bounds[2];
+  int before = 0, mine = 0;
   for (int base = 1; base <= n_groups; base += THREADS) {
     const int j = base + (int)threadIdx.x;
-    before += __syncthreads_count(j <= n_groups &&
-                                  group_begin(ptr, j, rows) / tile_rows + j <= slot);
+    mine = j <= n_groups ? group_begin(ptr, j, rows) : rows;
+    before += __syncthreads_count(j <= n_groups && mine / tile_rows + j <= slot);
   }
-  const int p0 = group_begin(ptr, before, rows);
+  int p0 = 0, p1 = rows;
+  if (n_groups <= THREADS) {
+    if ((int)threadIdx.x + 1 == before) bounds[0] = mine;
+    if ((int)threadIdx.x == before) bounds[1] = mine;       // (rows, behind the last group)
+    __syncthreads();
+    if (before > 0) p0 = bounds[0];
+    if (before < n_groups) p1 = bounds[1];
+  } else {
+    p0 = group_begin(ptr, before, rows);
+    if (before < n_groups) p1 = group_begin(ptr, before + 1, rows);
+  }
   *tile = slot - (p0 / tile_rows + before);
   *g = before;
   *first = p0 + *tile * tile_rows;
-  *end = before == n_groups ? rows : group_begin(ptr, before + 1, rows);
+  *end = p1;
   return *tile >= 0 && *first < *end;
 }
 
@@ -396,6 +409,19 @@ __device__ inline int row_at(const int *order, int r, int rows, int *err) {
   if ((unsigned)id < (unsigned)rows) return id;
   *err = 1;
   return -1;
+}
+
+// The row numbers of a tile, thread t's of row t: -1 behind the group's last row and (reported)
+// outside the matrix.
+template <int BM>
+__device__ inline void put_row_ids(int *row_ids, int mine, int first, int end, const GroupedArgs &a) {
+  const int t = threadIdx.x;
+  if (t < BM) {
+    const bool inside = (unsigned)mine < (unsigned)a.rows;
+    if (!inside && first + t < end) *a.err = 1;
+    row_ids[t] = inside && first + t < end ? mine : -1;
+  }
+  __syncthreads();
 }
 
 // Results of a wave's blocks, with the bias, into the rows of Y.
@@ -440,7 +466,7 @@ template <int D> struct RowsOut {
 };
 
 // ---- Y = X W + b -----------------------------------------------------------------------------------
-template <int D, int BM, int BN, int WM, int WN, bool TRANS_W, int STAGES>
+template <int D, int BM, int BN, int WM, int WN, bool TRANS_W, int STAGES, int FLIGHT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_kernel(const GroupedArgs a) {
   typedef typename Type<D>::Raw Raw;
   constexpr int T = 64 * WM * WN, BK = Type<D>::BK, P = Type<D>::P;
@@ -455,63 +481,86 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_kernel(const Gro
   if (!tile_of_slot<T>(a.ptr, a.n_groups, a.rows, BM, slot, &g, &first, &end, &tile)) return;
   const int tid = threadIdx.x, wave = tid >> 6;
   const int row0 = (wave / WN) * (BM / WM), col0 = (wave % WN) * (BN / WN);
-  for (int i = tid; i < BM; i += T)
-    row_ids[i] = first + i < end ? row_at(a.order, first + i, a.rows, a.err) : -1;
-  __syncthreads();
+  static_assert(BM <= T, "a row number to a thread");
+  const int my_row = a.order && tid < BM ? a.order[min(first + tid, end - 1)] : first + tid;
 
   f4 acc[MI][NJ] = {};
   const Raw *x = static_cast<const Raw *>(a.x);
   const Raw *w = static_cast<const Raw *>(a.w) + (long long)g * a.w_group;
   if (g < a.n_groups) {
     // (rows and columns outside the matrices repeat one inside; their results are dropped)
-    RowStage<D, BM, T> xs;
-    xs.init([&](int r) { return x + (long long)max(row_ids[r], 0) * a.ldx; });
-    RowStage<D, TRANS_W ? BN : 16, T> wr;
-    ColStage<D, TRANS_W ? 16 : BN, T> wc;
-    if constexpr (TRANS_W) wr.init([&](int c) { return w + (long long)min(n0 + c, a.n - 1) * a.ldw; });
+    RowStage<D, BM, T> xs[FLIGHT];
+    RowStage<D, TRANS_W ? BN : 16, T> wr[FLIGHT];
+    ColStage<D, TRANS_W ? 16 : BN, T> wc[FLIGHT];
+    if constexpr (TRANS_W)
+#pragma unroll
+      for (int f = 0; f < FLIGHT; f++)
+        wr[f].init([&](int c) { return w + (long long)min(n0 + c, a.n - 1) * a.ldw; });
     const int n_chunks = (a.k + BK - 1) / BK;
-    const bool whole_cols = wc.whole_vectors(n0, a.n);
-    auto load = [&](int c) __attribute__((always_inline)) {
+    const bool whole_cols = wc[0].whole_vectors(n0, a.n);
+    auto load_w = [&](int c, int f) __attribute__((always_inline)) {
       const int k0 = c * BK;
       const bool whole = k0 + BK <= a.k;
-      if (whole) xs.load(k0);
-      else xs.load_tail(k0, a.k);
       if constexpr (TRANS_W) {
-        if (whole) wr.load(k0);
-        else wr.load_tail(k0, a.k);
+        if (whole) wr[f].load(k0);
+        else wr[f].load_tail(k0, a.k);
       } else {
-        const int r0 = k0 + wc.row(), n = whole_cols ? wc.col_within(n0, a.n) : n0 + wc.col();
+        const int r0 = k0 + wc[f].row();
+        const int n = whole_cols ? wc[f].col_within(n0, a.n) : n0 + wc[f].col();
         const Raw *p = w + (long long)r0 * a.ldw + n;
-        if (whole && whole_cols && wc.active())
-          wc.load([&](int i) { return p + i * a.ldw; });
+        if (whole && whole_cols && wc[f].active())
+          wc[f].load([&](int i) { return p + i * a.ldw; });
         else
-          wc.load_tail(a.n - n, [&](int i) { return r0 + i < a.k ? p + i * a.ldw : nullptr; });
+          wc[f].load_tail(a.n - n, [&](int i) { return r0 + i < a.k ? p + i * a.ldw : nullptr; });
       }
     };
-    auto store = [&](int s) __attribute__((always_inline)) {
-      xs.store(xt + s * P * BM * BK);
-      if constexpr (TRANS_W) wr.store(wt + s * P * BN * BK);
-      else wc.store(wt + s * P * BN * BK);
+    auto load_x = [&](int c, int f) __attribute__((always_inline)) {
+      if (c * BK + BK <= a.k) xs[f].load(c * BK);
+      else xs[f].load_tail(c * BK, a.k);
     };
-    load(0);
+    auto load = [&](int c, int f) __attribute__((always_inline)) {
+      load_x(c, f);
+      load_w(c, f);
+    };
+    auto store = [&](int s, int f) __attribute__((always_inline)) {
+      xs[f].store(xt + s * P * BM * BK);
+      if constexpr (TRANS_W) wr[f].store(wt + s * P * BN * BK);
+      else wc[f].store(wt + s * P * BN * BK);
+    };
+    // (the first weights are on their way while the row numbers arrive, which the rows wait for)
+#pragma unroll
+    for (int f = 0; f < FLIGHT; f++)
+      if (f < n_chunks) load_w(f, f);
+    put_row_ids<BM>(row_ids, my_row, first, end, a);
+#pragma unroll
+    for (int f = 0; f < FLIGHT; f++) {
+      xs[f].init([&](int r) { return x + (long long)max(row_ids[r], 0) * a.ldx; });
+      if (f < n_chunks) load_x(f, f);
+    }
     if constexpr (STAGES == 2) {
-      store(0);
-      __syncthreads();
-      for (int c = 0; c < n_chunks; c++) {
-        if (c + 1 < n_chunks) load(c + 1);
-        multiply<D, BM, BN>(xt + (c & 1) * P * BM * BK, wt + (c & 1) * P * BN * BK, row0, col0, acc);
-        if (c + 1 < n_chunks) store((c + 1) & 1);
-        __syncthreads();
-      }
+      for (int c0 = 0; c0 < n_chunks; c0 += (FLIGHT > 1 ? FLIGHT : 2))
+#pragma unroll
+        for (int u = 0; u < (FLIGHT > 1 ? FLIGHT : 2); u++) {
+          const int c = c0 + u;
+          if (c >= n_chunks) break;
+          // (the other buffer may still be read; this one was read before the last barrier)
+          store(u & 1, u % FLIGHT);
+          __syncthreads();
+          if (c + FLIGHT < n_chunks) load(c + FLIGHT, u % FLIGHT);
+          multiply<D, BM, BN>(xt + (u & 1) * P * BM * BK, wt + (u & 1) * P * BN * BK, row0, col0, acc);
+        }
     } else {
+      static_assert(FLIGHT == 1, "one buffer, one chunk on its way");
       for (int c = 0; c < n_chunks; c++) {
         if (c > 0) __syncthreads();
-        store(0);
+        store(0, 0);
         __syncthreads();
-        if (c + 1 < n_chunks) load(c + 1);
+        if (c + 1 < n_chunks) load(c + 1, 0);
         multiply<D, BM, BN>(xt, wt, row0, col0, acc);
       }
     }
+  } else {
+    put_row_ids<BM>(row_ids, my_row, first, end, a);
   }
   const RowsOut<D> out{a, g};
   const int lane = tid & 63;
@@ -893,9 +942,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_lds_kernel(const
   if (!tile_of_slot<T>(a.ptr, a.n_groups, a.rows, BM, slot, &g, &first, &end, &tile)) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row0 = (wave / WN) * (BM / WM), col0 = (wave % WN) * (BN / WN);
-  for (int i = tid; i < BM; i += T)
-    row_ids[i] = first + i < end ? row_at(a.order, first + i, a.rows, a.err) : -1;
-  __syncthreads();
+  static_assert(BM <= T, "a row number to a thread");
+  put_row_ids<BM>(row_ids, a.order && tid < BM ? a.order[min(first + tid, end - 1)] : first + tid,
+                  first, end, a);
 
   Pipe pipe{};
   if (g < a.n_groups) {
@@ -1105,16 +1154,16 @@ template <int D> __global__ __launch_bounds__(256) void grouped_tn_finish_kernel
 }
 
 // ---- host side ---------------------------------------------------------------------------------------
-template <int D, int BM, int BN, int WM, int WN, int STAGES>
+template <int D, int BM, int BN, int WM, int WN, int STAGES, int FLIGHT>
 static int launch_rows_tile(GroupedArgs &a, bool trans_w, hipStream_t s) {
   a.n_tiles = (a.n + BN - 1) / BN;
   const int64_t blocks = ((int64_t)a.rows / BM + a.n_groups + 1) * a.n_tiles;
   INCAGG_REQUIRE(blocks < (1ll << 31), "too many rows and columns for one call");
   const dim3 grid((unsigned)blocks), block(64 * WM * WN);
   if (trans_w)
-    hipLaunchKernelGGL((grouped_rows_kernel<D, BM, BN, WM, WN, true, STAGES>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((grouped_rows_kernel<D, BM, BN, WM, WN, true, STAGES, FLIGHT>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((grouped_rows_kernel<D, BM, BN, WM, WN, false, STAGES>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((grouped_rows_kernel<D, BM, BN, WM, WN, false, STAGES, FLIGHT>), grid, block, 0, s, a);
   INCAGG_HIP_TRY(hipGetLastError());
   return INCAGG_OK;
 }
@@ -1153,9 +1202,9 @@ template <int D> static int launch_rows(GroupedArgs &a, bool trans_w, hipStream_
   constexpr int STAGES = D == INCAGG_DTYPE_F32 ? 1 : 2;
   // few rows to a group: the weights are what is read, and a tall tile would be mostly empty
   if ((int64_t)a.rows <= 48ll * a.n_groups)
-    return launch_rows_tile<D, 16, 64, 1, 4, STAGES>(a, trans_w, s);
-  if (a.n <= 64) return launch_rows_tile<D, 128, 64, 4, 1, STAGES>(a, trans_w, s);
-  return launch_rows_tile<D, 128, 128, 2, 2, STAGES>(a, trans_w, s);
+    return launch_rows_tile<D, 16, 64, 1, 4, 2, 4>(a, trans_w, s);
+  if (a.n <= 64) return launch_rows_tile<D, 128, 64, 4, 1, STAGES, 1>(a, trans_w, s);
+  return launch_rows_tile<D, 128, 128, 2, 2, STAGES, 1>(a, trans_w, s);
 }
 
 // Whether the weight gradient runs in 256 x 256 tiles where the operands' alignment allows it.

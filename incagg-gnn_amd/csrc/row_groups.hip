@@ -5,7 +5,7 @@
 //     ptr[g]  = number of rows with key < g,  g = 0 .. G
 //
 // A counting sort with ranks.  Every workgroup owns kChunk consecutive rows, every wave of it a
-// quarter of them.
+// quarter of them, eight to a lane, whose keys stay in registers from the count to the ranking.
 //   1. count:  keys per workgroup (LDS histogram)             -> table[key][workgroup]
 //   2. scan:   one workgroup per key, exclusive over workgroups, and the key's total
 //   3. place:  each workgroup scans the totals (where each key begins), adds its own offset, and
@@ -21,11 +21,11 @@
 
 namespace incagg {
 
-constexpr int kChunk = 4096;              // rows of a workgroup
+constexpr int kChunk = 2048;              // rows of a workgroup
 constexpr int kMaxGroups = 2048;       // (a counter per wave and key in LDS)
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kWaveRows = kChunk / kWaves;
+constexpr int kWaveRows = kChunk / kWaves, kLaneRows = kWaveRows / 64;
 
 // Key of a row; ids outside [-1, G) are reported and count as rows of no group.
 template <typename I> __device__ inline int key_of(I id, int n_groups, int *err) {
@@ -34,16 +34,32 @@ template <typename I> __device__ inline int key_of(I id, int n_groups, int *err)
   return n_groups;
 }
 
+// Keys of this lane's rows: rows begin + 64 j + lane, -1 behind the last.
+template <typename I>
+__device__ inline void load_keys(const I *ids, int begin, int end, int n_groups, int *err,
+                                 int (&key)[kLaneRows]) {
+  const int lane = threadIdx.x & 63;
+  I id[kLaneRows];
+#pragma unroll
+  for (int j = 0; j < kLaneRows; j++) id[j] = ids[min(begin + 64 * j + lane, end - 1)];
+#pragma unroll
+  for (int j = 0; j < kLaneRows; j++)
+    key[j] = begin + 64 * j + lane < end ? key_of(id[j], n_groups, err) : -1;
+}
+
 template <typename I>
 __global__ __launch_bounds__(kThreads) void count_kernel(const I *ids, int rows, int n_groups,
                                                          int n_blocks, int *table, int *err) {
   extern __shared__ int hist[];           // [n_groups + 1]
   const int n_keys = n_groups + 1;
+  const int begin = (int)blockIdx.x * kChunk + (int)(threadIdx.x >> 6) * kWaveRows;
+  int key[kLaneRows];
+  load_keys(ids, begin, rows, n_groups, err, key);
   for (int k = threadIdx.x; k < n_keys; k += kThreads) hist[k] = 0;
   __syncthreads();
-  const int begin = (int)blockIdx.x * kChunk, end = min(rows, begin + kChunk);
-  for (int i = begin + (int)threadIdx.x; i < end; i += kThreads)
-    atomicAdd(&hist[key_of(ids[i], n_groups, err)], 1);
+#pragma unroll
+  for (int j = 0; j < kLaneRows; j++)
+    if (key[j] >= 0) atomicAdd(&hist[key[j]], 1);
   __syncthreads();
   for (int k = threadIdx.x; k < n_keys; k += kThreads)
     table[(long long)k * n_blocks + blockIdx.x] = hist[k];
@@ -101,10 +117,14 @@ __global__ __launch_bounds__(kThreads) void place_kernel(const I *ids, int rows,
 
   // this wave's keys, counted
   int *mine = next + wave * n_keys;
+  int key[kLaneRows];
+  if (begin < end) load_keys(ids, begin, end, n_groups, err, key);
   for (int k = threadIdx.x; k < kWaves * n_keys; k += kThreads) next[k] = 0;
   __syncthreads();
-  for (int i = begin + lane; i < end; i += 64)
-    atomicAdd(&mine[key_of(ids[i], n_groups, err)], 1);
+  if (begin < end)
+#pragma unroll
+    for (int j = 0; j < kLaneRows; j++)
+      if (key[j] >= 0) atomicAdd(&mine[key[j]], 1);
   __syncthreads();
 
   // where each key begins, plus the rows of it in front of this workgroup and wave
@@ -134,23 +154,21 @@ __global__ __launch_bounds__(kThreads) void place_kernel(const I *ids, int rows,
   __syncthreads();
 
   // 64 rows at a time, in order: rank among the lanes of the same key
+  if (begin >= end) return;
   const unsigned long long below = (1ull << lane) - 1;
-  for (int first = begin; first < end; first += 64) {
-    const int i = first + lane;
-    const bool live = i < end;
-    const int key = live ? key_of(ids[i], n_groups, err) : 0;
+#pragma unroll
+  for (int j = 0; j < kLaneRows; j++) {
+    const bool live = key[j] >= 0;
     unsigned long long same = __ballot(live);
     for (int b = 0; b < key_bits; b++) {
-      const unsigned long long set = __ballot((key >> b) & 1);
-      same &= ((key >> b) & 1) ? set : ~set;
+      const unsigned long long set = __ballot((key[j] >> b) & 1);
+      same &= ((key[j] >> b) & 1) ? set : ~set;
     }
-    if (live) {
-      const int at = mine[key] + __popcll(same & below);
-      order[at] = i;
-    }
+    const bool leader = live && (same & below) == 0;
+    if (live) order[mine[key[j]] + __popcll(same & below)] = begin + 64 * j + lane;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (live && (same & below) == 0) mine[key] += __popcll(same);
+    if (leader) mine[key[j]] += __popcll(same);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }

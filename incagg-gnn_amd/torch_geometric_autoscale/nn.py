@@ -582,6 +582,11 @@ def grouped_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], groups: "o
     ops.group_rows / ops.groups_from_ptr); ``weight``: [n_groups, out, in], ``bias``:
     [n_groups, out] or ``None``.  Rows of no group give zeros, and get zero gradients.
     ``gathered``: a float32 result gets the row pitch an aggregation wants of its source."""
+    if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad
+                                           or (bias is not None and bias.requires_grad)):
+        out = ops.rows_empty(x.size(0), weight.size(1), x.device) \
+            if gathered and x.dtype == torch.float32 and x.is_cuda else None
+        return ops.grouped_gemm(x, weight, groups, trans_w=True, bias=bias, out=out)
     return _GroupedLinear.apply(x, weight, bias, groups, bool(gathered))
 
 

@@ -30,7 +30,7 @@ class _on_device:
 
     def __init__(self, device):
         idx = device.index
-        self._ctx = None if idx is None or idx == torch.cuda.current_device() \
+        self._ctx = None if idx is None or idx == torch._C._cuda_getDevice() \
             else torch.cuda.device(device)
 
     def __enter__(self):
@@ -44,7 +44,9 @@ class _on_device:
 
 
 def _stream_of(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # (torch.cuda.current_stream(device).cuda_stream without the Stream object: 0.2 us, not 2)
+    return torch._C._cuda_getCurrentRawStream(
+        torch._C._cuda_getDevice() if device.index is None else device.index)
 
 
 def _rows_f32(t: Tensor, name: str, device=None) -> None:
@@ -751,11 +753,16 @@ class RowGroups:
         return self.ptr.device
 
 
+_group_limit = None
+
+
 def _max_groups(n_groups: int) -> int:
+    global _group_limit
     n_groups = int(n_groups)
-    limit = lib().incagg_group_rows_max_groups()
-    if not 1 <= n_groups <= limit:
-        raise ValueError(f"n_groups must be between 1 and {limit}, got {n_groups}")
+    if _group_limit is None:
+        _group_limit = lib().incagg_group_rows_max_groups()
+    if not 1 <= n_groups <= _group_limit:
+        raise ValueError(f"n_groups must be between 1 and {_group_limit}, got {n_groups}")
     return n_groups
 
 
@@ -799,6 +806,10 @@ def groups_from_ptr(ptr: Tensor, n_rows: int) -> RowGroups:
 
 
 def _grouped_rows(t: Tensor, name: str, groups: RowGroups, dtype=None) -> None:
+    if (t.is_cuda and t.dim() == 2 and t.dtype in DTYPE_CODE and t.shape[0] == groups.n_rows
+            and t.shape[1] >= 1 and t.device == groups.device
+            and (dtype is None or t.dtype == dtype)):
+        return
     _need_cuda(t, name)
     if t.dtype not in DTYPE_CODE or (dtype is not None and t.dtype != dtype):
         raise TypeError(f"{name} must be " + (str(dtype) if dtype is not None else
@@ -807,14 +818,15 @@ def _grouped_rows(t: Tensor, name: str, groups: RowGroups, dtype=None) -> None:
         raise ValueError(f"{name} must be [{groups.n_rows}, width], got {tuple(t.shape)}")
     if t.device != groups.device:
         raise ValueError(f"{name} is on {t.device}, the groups are on {groups.device}")
-    if t.size(1) < 1:
-        raise ValueError(f"{name} has no columns")
+    raise ValueError(f"{name} has no columns")
 
 
 def _plain_rows(t: Tensor) -> Tensor:
     """``t``, or a copy of it where its rows are not unit-stride or overlap (an expanded
     gradient)."""
-    if (t.size(1) > 1 and t.stride(1) != 1) or (t.size(0) > 1 and t.stride(0) < t.size(1)):
+    rows, width = t.shape
+    pitch, unit = t.stride()
+    if (width > 1 and unit != 1) or (rows > 1 and pitch < width):
         return t.contiguous()
     return t
 
@@ -829,34 +841,38 @@ def grouped_gemm(x: Tensor, w: Tensor, groups: RowGroups, trans_w: bool = False,
     if w.dtype != dt or (bias is not None and bias.dtype != dt):
         raise TypeError(f"x, w and bias must have one dtype, got {dt}, {w.dtype}"
                         + ("" if bias is None else f", {bias.dtype}"))
-    if w.dim() != 3 or w.size(0) != groups.n_groups or w.size(2 if trans_w else 1) != x.size(1):
-        raise ValueError(f"w must be [{groups.n_groups}, "
-                         + ("n, " if trans_w else "") + f"{x.size(1)}"
+    rows, k = x.shape
+    n_groups = groups.n_groups
+    if w.dim() != 3 or w.shape[0] != n_groups or w.shape[2 if trans_w else 1] != k:
+        raise ValueError(f"w must be [{n_groups}, " + ("n, " if trans_w else "") + f"{k}"
                          + ("" if trans_w else ", n") + f"], got {tuple(w.shape)}")
-    n = w.size(1 if trans_w else 2)
+    n = w.shape[1 if trans_w else 2]
     if n < 1:
         raise ValueError("w has no columns")
     if w.device != dev or (bias is not None and bias.device != dev):
         raise ValueError("x, w and bias must be on one device")
-    if bias is not None and tuple(bias.shape) != (groups.n_groups, n):
-        raise ValueError(f"bias must be [{groups.n_groups}, {n}], got {tuple(bias.shape)}")
     x = _plain_rows(x)
-    if w.stride(2) != 1 or w.stride(1) < w.size(2) or w.stride(0) < 0:
+    w_group, ldw, unit = w.stride()
+    if unit != 1 or ldw < w.shape[2] or w_group < 0:
         w = w.contiguous()
-    if bias is not None and (bias.stride(1) != 1 or bias.stride(0) < n):
-        bias = bias.contiguous()
+        w_group, ldw, _ = w.stride()
+    ld_bias = 0
+    if bias is not None:
+        if tuple(bias.shape) != (n_groups, n):
+            raise ValueError(f"bias must be [{n_groups}, {n}], got {tuple(bias.shape)}")
+        bias = _plain_rows(bias)
+        ld_bias = _ld(bias)
     if out is None:
-        out = torch.empty((x.size(0), n), dtype=dt, device=dev)
+        out = torch.empty((rows, n), dtype=dt, device=dev)
     else:
         _grouped_rows(out, "out", groups, dt)
-        if out.size(1) != n or _plain_rows(out) is not out:
-            raise ValueError(f"out must be [{x.size(0)}, {n}] with unit-stride rows")
+        if out.shape[1] != n or _plain_rows(out) is not out:
+            raise ValueError(f"out must be [{rows}, {n}] with unit-stride rows")
     with _on_device(dev):
         check(lib().incagg_grouped_gemm(
-            _ptr(x), _ld(x), _ptr(w), w.stride(1), w.stride(0), 1 if trans_w else 0, _ptr(bias),
-            0 if bias is None else bias.stride(0), groups.ptr.data_ptr(), _ptr(groups.order),
-            groups.n_groups, groups.n_rows, x.size(1), n, DTYPE_CODE[dt], _ptr(out), _ld(out),
-            _stream_of(dev)))
+            _ptr(x), _ld(x), w.data_ptr(), ldw, w_group, 1 if trans_w else 0, _ptr(bias), ld_bias,
+            groups.ptr.data_ptr(), _ptr(groups.order), n_groups, rows, k, n, DTYPE_CODE[dt],
+            _ptr(out), _ld(out), _stream_of(dev)))
     return out
 
 

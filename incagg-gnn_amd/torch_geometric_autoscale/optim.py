@@ -35,51 +35,51 @@ def _max_norm(max_norm) -> float:
     return max_norm
 
 
-def _check_grad(g: Tensor, dev) -> None:
+def _refuse_grad(g: Tensor, like: Tensor) -> None:
     if not g.is_cuda:
         raise RuntimeError("gradients must live on the GPU: the norm and clipping kernels are HIP "
                            "only and there is no CPU implementation")
     if g.layout != torch.strided or g.dtype not in ops.DTYPE_CODE:
         raise TypeError(f"gradients must be dense float32, bfloat16 or float16, got {g.dtype}")
-    if g.device != dev:
+    if g.device != like.device:
         raise ValueError("all gradients must be on one device")
-
-
-def _norm_call(grads: List[Tensor], norm_type: int, max_norm: Optional[float]) -> Tensor:
-    """The norm of contiguous tensors (and their scaling, with ``max_norm``)."""
-    L, dev = _lib.lib(), grads[0].device
-    flat, total = [], 0
-    for g in grads:
-        n = g.numel()
-        total += n
-        flat += (g.data_ptr(), n, ops.DTYPE_CODE[g.dtype])
-    segs = array.array("q", flat)                   # incagg_norm_segment[]
-    need = L.incagg_grad_norm_ws_doubles(len(grads), total)
-    _lib.check(need)
-    ws = torch.empty(max(need, 1), dtype=torch.float64, device=dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    with ops._on_device(dev):
-        if max_norm is None:
-            _lib.check(L.incagg_grad_norm(segs.buffer_info()[0], len(grads), norm_type,
-                                          ws.data_ptr(), need, norm.data_ptr(),
-                                          ops._stream_of(dev)))
-        else:
-            _lib.check(L.incagg_grad_clip(segs.buffer_info()[0], len(grads), norm_type, max_norm,
-                                          ws.data_ptr(), need, norm.data_ptr(),
-                                          ops._stream_of(dev)))
-    return norm
 
 
 def _gradients(parameters) -> List[Tensor]:
     if isinstance(parameters, Tensor):
-        parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
-    for g in grads:
-        _check_grad(g, grads[0].device)
+        parameters = (parameters,)
+    code, strided = ops.DTYPE_CODE, torch.strided
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    if grads:
+        dev = grads[0].get_device()             # (-1: on the host)
+        for g in grads:
+            if g.get_device() != dev or dev < 0 or g.dtype not in code or g.layout != strided:
+                _refuse_grad(g, grads[0])
     return grads
 
 
-@torch.no_grad()
+def _norm_call(grads: List[Tensor], norm_type: int, max_norm: Optional[float]) -> Tensor:
+    """The norm of contiguous tensors (and their scaling, with ``max_norm``)."""
+    L, dev, code = _lib.lib(), grads[0].device, ops.DTYPE_CODE
+    flat = []
+    for g in grads:
+        flat += (g.data_ptr(), g.numel(), code[g.dtype])
+    segs = array.array("q", flat)                   # incagg_norm_segment[]
+    need = L.incagg_grad_norm_ws_doubles(len(grads), sum(flat[1::3]))
+    _lib.check(need)
+    ws = torch.empty(need + 1, dtype=torch.float64, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    args = (segs.buffer_info()[0], len(grads), norm_type)
+    with ops._on_device(dev):
+        stream = ops._stream_of(dev)
+        if max_norm is None:
+            _lib.check(L.incagg_grad_norm(*args, ws.data_ptr(), need, norm.data_ptr(), stream))
+        else:
+            _lib.check(L.incagg_grad_clip(*args, max_norm, ws.data_ptr(), need, norm.data_ptr(),
+                                          stream))
+    return norm
+
+
 def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
     """The norm of all gradients taken as one vector (a float32 scalar on their device;
     incagg_grad_norm): two launches whatever the number of tensors (up to 128), 64-bit sums in a
@@ -89,10 +89,10 @@ def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.
     grads = _gradients(parameters)
     if not grads:
         return torch.zeros(())
-    return _norm_call([g if g.is_contiguous() else g.contiguous() for g in grads], code, None)
+    return _norm_call([g if g.is_contiguous() else g.detach().contiguous() for g in grads], code,
+                      None)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
                     norm_type: float = 2.0, error_if_nonfinite: bool = False) -> Tensor:
     """``torch.nn.utils.clip_grad_norm_`` (main.py:82-84) in two launches: scales all gradients in
@@ -104,19 +104,22 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     grads = _gradients(parameters)
     if not grads:
         return torch.zeros(())
-    dense = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    copies = [(i, g) for i, g in enumerate(grads) if not g.is_contiguous()]
+    dense = grads
+    if copies:
+        dense = list(grads)
+        for i, g in copies:     # (refused before anything is scaled)
+            if 0 in g.stride() and g.numel() > 1:
+                raise RuntimeError("a gradient's elements overlap in memory (an expanded tensor)")
+            dense[i] = g.detach().contiguous()
     if error_if_nonfinite:
         norm = _norm_call(dense, code, None)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is "
                                "non-finite, so it cannot be clipped")
-    for g in grads:     # (before anything is scaled)
-        if not g.is_contiguous() and 0 in g.stride() and g.numel() > 1:
-            raise RuntimeError("a gradient's elements overlap in memory (an expanded tensor)")
     norm = _norm_call(dense, code, max_norm)
-    for g, d in zip(grads, dense):
-        if d is not g:
-            g.copy_(d)
+    for i, g in copies:
+        g.detach().copy_(dense[i])
     return norm
 
 
@@ -166,6 +169,8 @@ class Adam:
                                  "exp_avg_sq": flat[sum(sizes) + off:sum(sizes) + off + p.numel()]
                                  .view_as(p)}
                 off += n
+        # (the same dicts by position: a lookup by tensor costs a fifth of a small step)
+        self._states = [[self.state[p] for p in group["params"]] for group in self.param_groups]
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         for group in self.param_groups:
@@ -177,13 +182,16 @@ class Adam:
                 else:
                     p.grad.detach_().zero_()
 
-    @torch.no_grad()
     def step(self, max_norm: Optional[float] = None) -> Optional[Tensor]:
         """``max_norm``: the gradients are clipped by their global 2-norm (over all groups) as they
         are read -- ``clip_grad_norm_`` and the step in two launches; ``p.grad`` itself stays as
         it is -- and the norm they had is returned (a scalar on the device)."""
         if max_norm is not None:
             return self._clipped_step(_max_norm(max_norm))
+        return self._plain_step()
+
+    @torch.no_grad()
+    def _plain_step(self) -> None:
         L = _lib.lib()
         for group in self.param_groups:
             with_grad = [p for p in group["params"] if p.grad is not None]
@@ -209,31 +217,29 @@ class Adam:
                     group["weight_decay"], ops._stream_of(self.device)))
 
     def _clipped_step(self, max_norm: float) -> Tensor:
-        L, dev = _lib.lib(), self.device
-        flat, keep, total = [], [], 0
+        L, dev, f32, strided = _lib.lib(), self.device, torch.float32, torch.strided
+        flat, keep, index = [], [], dev.index
         hyper = (_lib.AdamHyper * len(self.param_groups))()
         for i, group in enumerate(self.param_groups):
             b1, b2 = group["betas"]
             hyper[i] = _lib.AdamHyper(group["lr"], b1, b2, group["eps"], group["weight_decay"])
-            for p in group["params"]:
+            for p, st in zip(group["params"], self._states[i]):
                 g = p.grad
                 if g is None:
                     continue
-                if g.dtype != torch.float32 or g.device != dev:
+                if g.dtype != f32 or g.get_device() != index or g.layout != strided:
                     raise TypeError("gradients must be float32 on the parameter's device")
                 if not g.is_contiguous():
-                    g = g.contiguous()
+                    g = g.detach().contiguous()
                     keep.append(g)
-                st, n = self.state[p], p.numel()
-                total += n
                 flat += (p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
-                         st["exp_avg_sq"].data_ptr(), st["step"].data_ptr(), n, i)
+                         st["exp_avg_sq"].data_ptr(), st["step"].data_ptr(), p.numel(), i)
         segs = array.array("q", flat)               # incagg_adam_clip_segment[]
         n_segs = len(flat) // 7
-        need = L.incagg_grad_norm_ws_doubles(n_segs, total)
+        need = L.incagg_grad_norm_ws_doubles(n_segs, sum(flat[5::7]))
         _lib.check(need)
-        ws = torch.empty(max(need, 1), dtype=torch.float64, device=dev)
-        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws = torch.empty(need + 1, dtype=torch.float64, device=dev)
+        norm = torch.empty((), dtype=f32, device=dev)
         with ops._on_device(dev):
             _lib.check(L.incagg_adam_step_clipped_f32(
                 segs.buffer_info()[0], n_segs, ctypes.addressof(hyper), len(hyper), max_norm,
