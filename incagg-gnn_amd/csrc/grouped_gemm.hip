@@ -1187,10 +1187,25 @@ static bool pieces(const void *p, int64_t ld, int64_t width) {
   return aligned16(p) && ld % 8 == 0 && width % 8 == 0;
 }
 
+// Tiles by the average number of rows to a group: below one tile of rows the weights are what is
+// read, and a tall tile is mostly empty.  64 groups, 1024 -> 1024 bfloat16 and 512 -> 512 float32,
+// forward, us by rows of a tile (128: the LDS-loading kernel for bfloat16):
+//     rows to a group      4     16     32     64    128    256    512
+//     bfloat16    16    24.3   28.0   33.5   53.5   86.4    148    283
+//                 64    26.1   27.4   28.3   39.1   46.0   70.1    124
+//                128    35.8   36.8   37.3   40.2   58.0   60.3   92.8
+//     float32     16    21.0   24.7   33.7   49.0   82.0    150    289
+//                 64    31.5   30.0   30.9   39.4   47.2   66.3    113
+//                128    44.0   43.1   43.6   44.2   46.9   75.8    120     (8192 rows: 941 / 881)
 template <int D> static int launch_rows(GroupedArgs &a, bool trans_w, hipStream_t s) {
-  if constexpr (D != INCAGG_DTYPE_F32) {
-    if ((int64_t)a.rows > 48ll * a.n_groups && a.n > 64 && pieces(a.x, a.ldx, a.k) &&
-        pieces(a.w, a.ldw, trans_w ? a.k : a.n) && a.w_group % 8 == 0) {
+  constexpr bool F32 = D == INCAGG_DTYPE_F32;
+  constexpr int STAGES = F32 ? 1 : 2;
+  const int64_t average = a.rows / a.n_groups;
+  if (average <= 16) return launch_rows_tile<D, 16, 64, 1, 4, 2, 4>(a, trans_w, s);
+  if (a.n <= 64) return launch_rows_tile<D, 128, 64, 4, 1, STAGES, 1>(a, trans_w, s);
+  if (average <= (F32 ? 768 : 64)) return launch_rows_tile<D, 64, 128, 2, 2, STAGES, 1>(a, trans_w, s);
+  if constexpr (!F32) {
+    if (pieces(a.x, a.ldx, a.k) && pieces(a.w, a.ldw, trans_w ? a.k : a.n) && a.w_group % 8 == 0) {
       // 256 x 256 halves what a tile reads for its products, but leaves one workgroup to a CU: for
       // at least one round of them (128 x 128 against it, 131072 x 1024 -> 2048: 848 / 671 us,
       // 32768 x 1024 -> 1024, two rounds: 93 / 90 us)
@@ -1199,11 +1214,6 @@ template <int D> static int launch_rows(GroupedArgs &a, bool trans_w, hipStream_
       return launch_rows_lds<D, 256, 256, 2, 4>(a, trans_w, s);
     }
   }
-  constexpr int STAGES = D == INCAGG_DTYPE_F32 ? 1 : 2;
-  // few rows to a group: the weights are what is read, and a tall tile would be mostly empty
-  if ((int64_t)a.rows <= 48ll * a.n_groups)
-    return launch_rows_tile<D, 16, 64, 1, 4, 2, 4>(a, trans_w, s);
-  if (a.n <= 64) return launch_rows_tile<D, 128, 64, 4, 1, STAGES, 1>(a, trans_w, s);
   return launch_rows_tile<D, 128, 128, 2, 2, STAGES, 1>(a, trans_w, s);
 }
 
