@@ -6,7 +6,10 @@
 // the way the reference asserts them (csrc/cuda/async_cuda.cu:20-59,119-137,
 // csrc/cpu/relabel_cpu.cpp:9-16) and unwrapped into pointers and sizes.
 //
-// One source, two objects: -DINCAGG_OPS_RELABEL builds `_relabel`, -DINCAGG_OPS_ASYNC `_async`.
+// One source, three objects: -DINCAGG_OPS_RELABEL builds `_relabel`, -DINCAGG_OPS_ASYNC `_async`;
+// -DINCAGG_OPS_GRADS builds `_grads`, which has no counterpart in the reference: gradient lists
+// (norm, clipping, the clipped Adam step) handed to the C ABI without a Python loop over the
+// tensors -- a list of ten took longer to walk there than the GPU needs for the whole call.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -190,8 +193,138 @@ void write_async(Tensor src, Tensor offset, Tensor count, Tensor dst) {
 }
 #endif  // INCAGG_OPS_ASYNC
 
+#ifdef INCAGG_OPS_GRADS
+int64_t element_code(const Tensor &t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return INCAGG_DTYPE_F32;
+    case at::kBFloat16: return INCAGG_DTYPE_BF16;
+    case at::kHalf: return INCAGG_DTYPE_F16;
+    default: return -1;
+  }
+}
+
+// The gradients as segments; those that are not contiguous as copies (`dense`), which are written
+// back behind the call when `scaled`.
+struct Segments {
+  std::vector<incagg_norm_segment> segs;
+  std::vector<std::pair<size_t, Tensor>> dense;
+  int64_t elements = 0;
+
+  Segments(const std::vector<Tensor> &grads, bool scaled) {
+    segs.reserve(grads.size());
+    for (size_t i = 0; i < grads.size(); i++) {
+      const Tensor &g = grads[i];
+      TORCH_CHECK(g.is_cuda(), "gradients must live on the GPU: the norm and clipping kernels are "
+                  "HIP only and there is no CPU implementation");
+      const int64_t code = g.layout() == at::kStrided ? element_code(g) : -1;
+      TORCH_CHECK_TYPE(code >= 0, "gradients must be dense float32, bfloat16 or float16, got ",
+                       g.scalar_type());
+      TORCH_CHECK_VALUE(g.device() == grads[0].device(), "all gradients must be on one device");
+      void *p = g.numel() ? g.data_ptr() : nullptr;
+      if (!g.is_contiguous()) {
+        if (scaled && g.numel() > 1)
+          for (int64_t st : g.strides())
+            TORCH_CHECK(st != 0, "a gradient's elements overlap in memory (an expanded tensor)");
+        dense.emplace_back(i, g.detach().contiguous());
+        p = dense.back().second.data_ptr();
+      }
+      segs.push_back({p, g.numel(), code});
+      elements += g.numel();
+    }
+  }
+};
+
+struct Scratch {
+  Tensor ws, norm;
+  int64_t doubles;
+  Scratch(int64_t n_segs, int64_t elements, const at::Device &device)
+      : doubles(incagg_grad_norm_ws_doubles(n_segs, elements)) {
+    check_status(doubles);
+    const auto options = at::TensorOptions().device(device);
+    ws = at::empty({doubles + 1}, options.dtype(at::kDouble));
+    norm = at::empty({}, options.dtype(at::kFloat));
+  }
+  double *ptr() { return ws.data_ptr<double>(); }
+};
+
+void *current_stream(const at::Device &device) {
+  return c10::hip::getCurrentHIPStream(device.index()).stream();
+}
+
+Tensor grad_norm(std::vector<Tensor> grads, int64_t norm_type, double max_norm, bool clip) {
+  TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
+  const Segments s(grads, clip);
+  const at::Device device = grads[0].device();
+  c10::DeviceGuard guard(device);
+  const int64_t n = (int64_t)s.segs.size();
+  Scratch scratch(n, s.elements, device);
+  float *out = scratch.norm.data_ptr<float>();
+  if (!clip) {
+    check_status(incagg_grad_norm(s.segs.data(), n, (int)norm_type, scratch.ptr(), scratch.doubles,
+                                  out, current_stream(device)));
+    return scratch.norm;
+  }
+  check_status(incagg_grad_clip(s.segs.data(), n, (int)norm_type, max_norm, scratch.ptr(),
+                                scratch.doubles, out, current_stream(device)));
+  for (const auto &d : s.dense) grads[d.first].detach().copy_(d.second);
+  return scratch.norm;
+}
+
+// hyper: lr, beta1, beta2, eps, weight_decay of every parameter group; group[i]: of tensor i.
+Tensor adam_step_clipped(std::vector<Tensor> params, std::vector<Tensor> grads,
+                         std::vector<Tensor> exp_avg, std::vector<Tensor> exp_avg_sq,
+                         std::vector<Tensor> steps, std::vector<int64_t> group,
+                         std::vector<double> hyper, double max_norm, at::Device device) {
+  const size_t n = params.size();
+  TORCH_CHECK_VALUE(grads.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n &&
+                    steps.size() == n && group.size() == n && hyper.size() % 5 == 0,
+                    "one gradient, two moments, a step count and a group for every parameter");
+  std::vector<incagg_adam_clip_segment> segs;
+  std::vector<Tensor> keep;
+  segs.reserve(n);
+  int64_t elements = 0;
+  auto state = [&](const Tensor &t, int64_t numel) {
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat && t.device() == device,
+                     "parameters and state must be float32 on one device");
+    TORCH_CHECK_VALUE(t.is_contiguous() && t.numel() == numel,
+                      "parameters and state must be contiguous and of one size");
+    return numel ? static_cast<float *>(t.data_ptr()) : nullptr;
+  };
+  for (size_t i = 0; i < n; i++) {
+    Tensor g = grads[i];
+    TORCH_CHECK_TYPE(g.layout() == at::kStrided && g.scalar_type() == at::kFloat &&
+                     g.device() == device, "gradients must be float32 on the parameter's device");
+    const int64_t numel = params[i].numel();
+    TORCH_CHECK_VALUE(g.numel() == numel, "a gradient differs in size from its parameter");
+    if (!g.is_contiguous()) {
+      g = g.detach().contiguous();
+      keep.push_back(g);
+    }
+    segs.push_back({state(params[i], numel), numel ? static_cast<const float *>(g.data_ptr()) : nullptr,
+                    state(exp_avg[i], numel), state(exp_avg_sq[i], numel), state(steps[i], 1), numel,
+                    group[i]});
+    elements += numel;
+  }
+  c10::DeviceGuard guard(device);
+  Scratch scratch((int64_t)n, elements, device);
+  check_status(incagg_adam_step_clipped_f32(
+      segs.data(), (int64_t)n, reinterpret_cast<const incagg_adam_hyper *>(hyper.data()),
+      (int64_t)(hyper.size() / 5), max_norm, scratch.ptr(), scratch.doubles,
+      scratch.norm.data_ptr<float>(), current_stream(device)));
+  return scratch.norm;
+}
+#endif  // INCAGG_OPS_GRADS
+
 }  // namespace
 
+#ifdef INCAGG_OPS_GRADS
+TORCH_LIBRARY(incagg_grads, m) {
+  m.def("grad_norm(Tensor[] grads, int norm_type, float max_norm, bool clip) -> Tensor", &grad_norm);
+  m.def("adam_step_clipped(Tensor[] params, Tensor[] grads, Tensor[] exp_avg, Tensor[] exp_avg_sq, "
+        "Tensor[] steps, int[] group, float[] hyper, float max_norm, Device device) -> Tensor",
+        &adam_step_clipped);
+}
+#else
 // Both objects contribute to one namespace, hence fragments.
 TORCH_LIBRARY_FRAGMENT(torch_geometric_autoscale, m) {
 #ifdef INCAGG_OPS_RELABEL
@@ -207,3 +340,4 @@ TORCH_LIBRARY_FRAGMENT(torch_geometric_autoscale, m) {
   m.def("write_async(Tensor src, Tensor offset, Tensor count, Tensor dst) -> ()", &write_async);
 #endif
 }
+#endif

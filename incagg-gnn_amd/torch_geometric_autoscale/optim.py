@@ -9,8 +9,8 @@ advances the step counters); this one gives every 1 024 elements a workgroup.  T
 (one per parameter, as in torch) live on the device and are advanced there, so a step recorded
 into a HIP graph keeps counting when it is replayed.
 """
-import array
 import ctypes
+import os
 from typing import Iterable, List, Optional, Union
 
 import torch
@@ -35,49 +35,28 @@ def _max_norm(max_norm) -> float:
     return max_norm
 
 
-def _refuse_grad(g: Tensor, like: Tensor) -> None:
-    if not g.is_cuda:
-        raise RuntimeError("gradients must live on the GPU: the norm and clipping kernels are HIP "
-                           "only and there is no CPU implementation")
-    if g.layout != torch.strided or g.dtype not in ops.DTYPE_CODE:
-        raise TypeError(f"gradients must be dense float32, bfloat16 or float16, got {g.dtype}")
-    if g.device != like.device:
-        raise ValueError("all gradients must be on one device")
+_ops = None
+
+
+def _grad_ops():
+    """The operator object that walks gradient lists (`_grads.so`, csrc/build_torch_ops.py)."""
+    global _ops
+    if _ops is None:
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_grads.so")
+        if not os.path.isfile(path):
+            raise _lib.IncAggLibraryError(
+                f"{path} not found: build it with `python incagg-gnn_amd/csrc/build_torch_ops.py` "
+                "(there is no fallback implementation)")
+        torch.ops.load_library(path)
+        ns = torch.ops.incagg_grads
+        _ops = (ns.grad_norm.default, ns.adam_step_clipped.default)
+    return _ops
 
 
 def _gradients(parameters) -> List[Tensor]:
     if isinstance(parameters, Tensor):
         parameters = (parameters,)
-    code, strided = ops.DTYPE_CODE, torch.strided
-    grads = [g for g in [p.grad for p in parameters] if g is not None]
-    if grads:
-        dev = grads[0].get_device()             # (-1: on the host)
-        for g in grads:
-            if g.get_device() != dev or dev < 0 or g.dtype not in code or g.layout != strided:
-                _refuse_grad(g, grads[0])
-    return grads
-
-
-def _norm_call(grads: List[Tensor], norm_type: int, max_norm: Optional[float]) -> Tensor:
-    """The norm of contiguous tensors (and their scaling, with ``max_norm``)."""
-    L, dev, code = _lib.lib(), grads[0].device, ops.DTYPE_CODE
-    flat = []
-    for g in grads:
-        flat += (g.data_ptr(), g.numel(), code[g.dtype])
-    segs = array.array("q", flat)                   # incagg_norm_segment[]
-    need = L.incagg_grad_norm_ws_doubles(len(grads), sum(flat[1::3]))
-    _lib.check(need)
-    ws = torch.empty(need + 1, dtype=torch.float64, device=dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    args = (segs.buffer_info()[0], len(grads), norm_type)
-    with ops._on_device(dev):
-        stream = ops._stream_of(dev)
-        if max_norm is None:
-            _lib.check(L.incagg_grad_norm(*args, ws.data_ptr(), need, norm.data_ptr(), stream))
-        else:
-            _lib.check(L.incagg_grad_clip(*args, max_norm, ws.data_ptr(), need, norm.data_ptr(),
-                                          stream))
-    return norm
+    return [g for g in [p.grad for p in parameters] if g is not None]
 
 
 def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
@@ -87,10 +66,7 @@ def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.
     ``inf``."""
     code = _norm_type(norm_type)
     grads = _gradients(parameters)
-    if not grads:
-        return torch.zeros(())
-    return _norm_call([g if g.is_contiguous() else g.detach().contiguous() for g in grads], code,
-                      None)
+    return _grad_ops()[0](grads, code, 0.0, False) if grads else torch.zeros(())
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
@@ -104,23 +80,11 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     grads = _gradients(parameters)
     if not grads:
         return torch.zeros(())
-    copies = [(i, g) for i, g in enumerate(grads) if not g.is_contiguous()]
-    dense = grads
-    if copies:
-        dense = list(grads)
-        for i, g in copies:     # (refused before anything is scaled)
-            if 0 in g.stride() and g.numel() > 1:
-                raise RuntimeError("a gradient's elements overlap in memory (an expanded tensor)")
-            dense[i] = g.detach().contiguous()
-    if error_if_nonfinite:
-        norm = _norm_call(dense, code, None)
-        if not bool(torch.isfinite(norm)):
-            raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is "
-                               "non-finite, so it cannot be clipped")
-    norm = _norm_call(dense, code, max_norm)
-    for i, g in copies:
-        g.detach().copy_(dense[i])
-    return norm
+    call = _grad_ops()[0]
+    if error_if_nonfinite and not bool(torch.isfinite(call(grads, code, 0.0, False))):
+        raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is "
+                           "non-finite, so it cannot be clipped")
+    return call(grads, code, max_norm, True)
 
 
 class Adam:
@@ -217,34 +181,20 @@ class Adam:
                     group["weight_decay"], ops._stream_of(self.device)))
 
     def _clipped_step(self, max_norm: float) -> Tensor:
-        L, dev, f32, strided = _lib.lib(), self.device, torch.float32, torch.strided
-        flat, keep, index = [], [], dev.index
-        hyper = (_lib.AdamHyper * len(self.param_groups))()
+        params, states, group_of, hyper = [], [], [], []
         for i, group in enumerate(self.param_groups):
-            b1, b2 = group["betas"]
-            hyper[i] = _lib.AdamHyper(group["lr"], b1, b2, group["eps"], group["weight_decay"])
-            for p, st in zip(group["params"], self._states[i]):
-                g = p.grad
-                if g is None:
-                    continue
-                if g.dtype != f32 or g.get_device() != index or g.layout != strided:
-                    raise TypeError("gradients must be float32 on the parameter's device")
-                if not g.is_contiguous():
-                    g = g.detach().contiguous()
-                    keep.append(g)
-                flat += (p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
-                         st["exp_avg_sq"].data_ptr(), st["step"].data_ptr(), p.numel(), i)
-        segs = array.array("q", flat)               # incagg_adam_clip_segment[]
-        n_segs = len(flat) // 7
-        need = L.incagg_grad_norm_ws_doubles(n_segs, sum(flat[5::7]))
-        _lib.check(need)
-        ws = torch.empty(need + 1, dtype=torch.float64, device=dev)
-        norm = torch.empty((), dtype=f32, device=dev)
-        with ops._on_device(dev):
-            _lib.check(L.incagg_adam_step_clipped_f32(
-                segs.buffer_info()[0], n_segs, ctypes.addressof(hyper), len(hyper), max_norm,
-                ws.data_ptr(), need, norm.data_ptr(), ops._stream_of(dev)))
-        return norm
+            hyper += (group["lr"], *group["betas"], group["eps"], group["weight_decay"])
+            params += group["params"]
+            states += self._states[i]
+            group_of += [i] * len(group["params"])
+        grads = [p.grad for p in params]
+        if any(g is None for g in grads):
+            live = [k for k, g in enumerate(grads) if g is not None]
+            params, states, group_of, grads = ([v[k] for k in live]
+                                               for v in (params, states, group_of, grads))
+        return _grad_ops()[1](params, grads, [st["exp_avg"] for st in states],
+                              [st["exp_avg_sq"] for st in states], [st["step"] for st in states],
+                              group_of, hyper, max_norm, self.device)
 
     def state_dict(self) -> dict:
         return {"param_groups": [{k: (v.clone() if isinstance(v, Tensor) else v)
