@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Builds the two operator objects the reference package loads by name
 (torch_geometric_autoscale/__init__.py:8-10): ``_relabel.so`` and ``_async.so``, next to this
-package's ``__init__``, and ``_grads.so``, this package's own (gradient lists).  All are thin shells over libincagg_gnn.so (csrc/torch_ops.cpp), built
+package's ``__init__``, and ``_train_ops.so``, this package's own (gradient lists, the grouped linear layer).  All are thin shells over libincagg_gnn.so (csrc/torch_ops.cpp), built
 with the host compiler against the installed torch headers; no GPU is needed to build or load
 them.  Usage: python build_torch_ops.py [--force]"""
 import os
@@ -15,7 +15,7 @@ PKG = os.path.join(os.path.dirname(HERE), "torch_geometric_autoscale")
 LIB_DIR = os.path.join(os.path.dirname(HERE), "lib")
 SRC = os.path.join(HERE, "torch_ops.cpp")
 TARGETS = {"_relabel": "INCAGG_OPS_RELABEL", "_async": "INCAGG_OPS_ASYNC",
-           "_grads": "INCAGG_OPS_GRADS"}
+           "_train_ops": "INCAGG_OPS_TRAIN"}
 
 
 def output(name: str) -> str:

@@ -7,13 +7,18 @@
 // csrc/cpu/relabel_cpu.cpp:9-16) and unwrapped into pointers and sizes.
 //
 // One source, three objects: -DINCAGG_OPS_RELABEL builds `_relabel`, -DINCAGG_OPS_ASYNC `_async`;
-// -DINCAGG_OPS_GRADS builds `_grads`, which has no counterpart in the reference: gradient lists
-// (norm, clipping, the clipped Adam step) handed to the C ABI without a Python loop over the
-// tensors -- a list of ten took longer to walk there than the GPU needs for the whole call.
+// -DINCAGG_OPS_TRAIN builds `_train_ops`, which has no counterpart in the reference: calls whose
+// kernels are shorter than their host side would be in Python -- gradient lists (norm, clipping, the
+// clipped Adam step: a list of ten took longer to walk than the GPU needs for the whole call) and
+// the grouped linear layer with its autograd node.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
+#ifdef INCAGG_OPS_TRAIN
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#endif
 
 #include <deque>
 #include <mutex>
@@ -193,7 +198,7 @@ void write_async(Tensor src, Tensor offset, Tensor count, Tensor dst) {
 }
 #endif  // INCAGG_OPS_ASYNC
 
-#ifdef INCAGG_OPS_GRADS
+#ifdef INCAGG_OPS_TRAIN
 int64_t element_code(const Tensor &t) {
   switch (t.scalar_type()) {
     case at::kFloat: return INCAGG_DTYPE_F32;
@@ -313,16 +318,144 @@ Tensor adam_step_clipped(std::vector<Tensor> params, std::vector<Tensor> grads,
       scratch.norm.data_ptr<float>(), current_stream(device)));
   return scratch.norm;
 }
-#endif  // INCAGG_OPS_GRADS
+
+// ---- the grouped linear layer ------------------------------------------------------------------
+// Rows as the C ABI takes them: unit stride, no two rows in one place (an expanded gradient).
+Tensor plain_rows(const Tensor &t) {
+  const bool unit = t.size(1) <= 1 || t.stride(1) == 1;
+  const bool apart = t.size(0) <= 1 || t.stride(0) >= t.size(1);
+  return unit && apart ? t : t.contiguous();
+}
+
+int64_t pitch_of(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : std::max<int64_t>(t.size(1), 1); }
+
+// [rows, width] with `pitch` elements from row to row (0: width).
+Tensor rows_empty(int64_t rows, int64_t width, int64_t pitch, const Tensor &like) {
+  if (pitch <= width) return at::empty({rows, width}, like.options());
+  return at::empty_strided({rows, width}, {pitch, 1}, like.options());
+}
+
+struct Groups {
+  Tensor ptr, order;                    // order undefined: the rows lie sorted
+  int64_t count() const { return ptr.numel() - 1; }
+  const int32_t *ptr_data() const { return ptr.data_ptr<int32_t>(); }
+  const int32_t *order_data() const {
+    return order.defined() && order.numel() ? order.data_ptr<int32_t>() : nullptr;
+  }
+};
+
+Tensor grouped_gemm(const Tensor &x_in, const Tensor &w_in, bool trans_w, const Tensor &bias_in,
+                    const Groups &groups, int64_t pitch) {
+  const Tensor x = plain_rows(x_in);
+  const bool plain = w_in.stride(2) == 1 && w_in.stride(1) >= w_in.size(2);
+  const Tensor w = plain ? w_in : w_in.contiguous();
+  const Tensor bias = bias_in.defined() ? plain_rows(bias_in) : bias_in;
+  const int64_t rows = x.size(0), k = x.size(1), n = w.size(trans_w ? 1 : 2);
+  Tensor y = rows_empty(rows, n, pitch, x);
+  c10::DeviceGuard guard(x.device());
+  check_status(incagg_grouped_gemm(
+      ptr_or_null<void>(x), pitch_of(x), w.data_ptr(), w.stride(1), w.stride(0), trans_w ? 1 : 0,
+      bias.defined() ? bias.data_ptr() : nullptr, bias.defined() ? pitch_of(bias) : 0,
+      groups.ptr_data(), groups.order_data(), groups.count(), rows, k, n, (int)element_code(x),
+      const_cast<void *>(ptr_or_null<void>(y)), pitch_of(y), current_stream(x.device())));
+  return y;
+}
+
+std::pair<Tensor, Tensor> grouped_tn(const Tensor &a_in, const Tensor &b_in, const Groups &groups,
+                                     bool sums) {
+  const Tensor a = plain_rows(a_in), b = plain_rows(b_in);
+  const int64_t rows = a.size(0), m = a.size(1), n = b.size(1), g = groups.count();
+  const int code = (int)element_code(a);
+  const int64_t need = incagg_grouped_tn_ws_bytes(g, rows, m, n, code);
+  check_status(need);
+  Tensor d = at::empty({g, m, n}, a.options()), s, ws;
+  if (sums) s = at::empty({g, m}, a.options());
+  if (need) ws = at::empty({need}, a.options().dtype(at::kByte));
+  c10::DeviceGuard guard(a.device());
+  check_status(incagg_grouped_tn(
+      ptr_or_null<void>(a), pitch_of(a), ptr_or_null<void>(b), pitch_of(b), groups.ptr_data(),
+      groups.order_data(), g, rows, m, n, code, d.data_ptr(), m * n, sums ? s.data_ptr() : nullptr,
+      need ? ws.data_ptr() : nullptr, need, current_stream(a.device())));
+  return {d, s};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w,
+                        const std::optional<Tensor> &bias, const Tensor &ptr,
+                        const std::optional<Tensor> &order, int64_t pitch_y, int64_t pitch_dx) {
+    const Groups groups{ptr, order.value_or(Tensor())};
+    ctx->save_for_backward({x, w, ptr, groups.order});
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["pitch"] = pitch_dx;
+    return grouped_gemm(x, w, true, bias.value_or(Tensor()), groups, pitch_y);
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor x = saved[0], w = saved[1], dy = grads[0];
+    const Groups groups{saved[2], saved[3]};
+    const bool has_bias = ctx->saved_data["bias"].toBool();
+    const bool need_w = ctx->needs_input_grad(1), need_b = has_bias && ctx->needs_input_grad(2);
+    variable_list out(7);
+    {
+      at::AutoGradMode no_graph(false);
+      if (ctx->needs_input_grad(0))
+        out[0] = grouped_gemm(dy, w, false, Tensor(), groups, ctx->saved_data["pitch"].toInt());
+      if (need_w || need_b) {
+        const auto d = grouped_tn(dy, x, groups, need_b);
+        if (need_w) out[1] = d.first;
+        if (need_b) out[2] = d.second;
+      }
+    }
+    if (!at::GradMode::is_enabled()) return out;
+    // a graph of the gradients was asked for: differentiating them again raises
+    for (int i = 0; i < 3; i++) {
+      if (!out[i].defined()) continue;
+      auto error = std::make_shared<torch::autograd::DelayedError>(
+          "the grouped linear layer has no second derivatives", 1);
+      Tensor t = out[i].detach();
+      t.set_requires_grad(true);
+      out[i] = (*error)({t})[0];
+    }
+    return out;
+  }
+};
+
+Tensor grouped_linear(const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias,
+                      const Tensor &ptr, const std::optional<Tensor> &order, int64_t n_rows,
+                      int64_t pitch_y, int64_t pitch_dx) {
+  TORCH_CHECK(x.is_cuda(), "x must live on the GPU: the grouped products are HIP only and there is "
+              "no CPU implementation");
+  TORCH_CHECK_TYPE(element_code(x) >= 0 && w.scalar_type() == x.scalar_type() &&
+                   (!bias || bias->scalar_type() == x.scalar_type()),
+                   "x, weight and bias must be of one dtype: float32, bfloat16 or float16");
+  TORCH_CHECK_VALUE(x.device() == ptr.device() && w.device() == x.device() &&
+                    (!bias || bias->device() == x.device()),
+                    "x, weight, bias and groups must be on one device");
+  const int64_t g = ptr.numel() - 1;
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == n_rows && x.size(1) >= 1, "x must be [", n_rows,
+                    ", in], got ", x.sizes());
+  TORCH_CHECK_VALUE(w.dim() == 3 && w.size(0) == g && w.size(1) >= 1 && w.size(2) == x.size(1),
+                    "weight must be [", g, ", out, ", x.size(1), "], got ", w.sizes());
+  TORCH_CHECK_VALUE(!bias || (bias->dim() == 2 && bias->size(0) == g && bias->size(1) == w.size(1)),
+                    "bias must be [", g, ", ", w.size(1), "]");
+  return GroupedLinear::apply(x, w, bias, ptr, order, pitch_y, pitch_dx);
+}
+#endif  // INCAGG_OPS_TRAIN
 
 }  // namespace
 
-#ifdef INCAGG_OPS_GRADS
-TORCH_LIBRARY(incagg_grads, m) {
+#ifdef INCAGG_OPS_TRAIN
+TORCH_LIBRARY(incagg_train, m) {
   m.def("grad_norm(Tensor[] grads, int norm_type, float max_norm, bool clip) -> Tensor", &grad_norm);
   m.def("adam_step_clipped(Tensor[] params, Tensor[] grads, Tensor[] exp_avg, Tensor[] exp_avg_sq, "
         "Tensor[] steps, int[] group, float[] hyper, float max_norm, Device device) -> Tensor",
         &adam_step_clipped);
+  m.def("grouped_linear(Tensor x, Tensor weight, Tensor? bias, Tensor ptr, Tensor? order, int n_rows, "
+        "int pitch_y, int pitch_dx) -> Tensor", &grouped_linear);
 }
 #else
 // Both objects contribute to one namespace, hence fragments.

@@ -548,46 +548,17 @@ class RowsLinear(Linear):
         return _RowsLinear.apply(x, self.weight, self.bias, self.gathered)
 
 
-class _GroupedLinear(torch.autograd.Function):
-    """``y[i] = x[i] @ W[g(i)]^T + b[g(i)]`` over rows of several groups."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, gathered):
-        ctx.save_for_backward(x, weight)
-        ctx.groups, ctx.has_bias = groups, bias is not None
-        ctx.gathered = gathered and x.dtype == torch.float32
-        out = ops.rows_empty(x.size(0), weight.size(1), x.device) if ctx.gathered else None
-        return ops.grouped_gemm(x, weight, groups, trans_w=True, bias=bias, out=out)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight = ctx.saved_tensors
-        need, groups = ctx.needs_input_grad, ctx.groups
-        dx = dw = db = None
-        if need[0]:
-            out = ops.rows_empty(x.size(0), x.size(1), x.device) if ctx.gathered else None
-            dx = ops.grouped_gemm(dy, weight, groups, out=out)
-        if need[1] or (ctx.has_bias and need[2]):
-            with_bias = ctx.has_bias and need[2]
-            dw = ops.grouped_tn(dy, x, groups, column_sums=with_bias)
-            if with_bias:
-                dw, db = dw
-        return dx, dw if need[1] else None, db, None, None
-
-
 def grouped_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], groups: "ops.RowGroups",
                    gathered: bool = False) -> Tensor:
     """``x[i] @ weight[g]^T + bias[g]`` for every row ``i``, ``g`` its group (``groups``:
     ops.group_rows / ops.groups_from_ptr); ``weight``: [n_groups, out, in], ``bias``:
     [n_groups, out] or ``None``.  Rows of no group give zeros, and get zero gradients.
     ``gathered``: a float32 result gets the row pitch an aggregation wants of its source."""
-    if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad
-                                           or (bias is not None and bias.requires_grad)):
-        out = ops.rows_empty(x.size(0), weight.size(1), x.device) \
-            if gathered and x.dtype == torch.float32 and x.is_cuda else None
-        return ops.grouped_gemm(x, weight, groups, trans_w=True, bias=bias, out=out)
-    return _GroupedLinear.apply(x, weight, bias, groups, bool(gathered))
+    pitch = dx_pitch = 0
+    if gathered and x.dtype == torch.float32 and x.dim() == 2 and weight.dim() == 3:
+        pitch, dx_pitch = ops.row_pitch(weight.shape[1]), ops.row_pitch(x.shape[1])
+    return ops.train_ops().grouped_linear(x, weight, bias, groups.ptr, groups.order, groups.n_rows,
+                                          pitch, dx_pitch)
 
 
 class GroupedLinear(torch.nn.Module):

@@ -10,7 +10,6 @@ advances the step counters); this one gives every 1 024 elements a workgroup.  T
 into a HIP graph keeps counting when it is replayed.
 """
 import ctypes
-import os
 from typing import Iterable, List, Optional, Union
 
 import torch
@@ -35,24 +34,6 @@ def _max_norm(max_norm) -> float:
     return max_norm
 
 
-_ops = None
-
-
-def _grad_ops():
-    """The operator object that walks gradient lists (`_grads.so`, csrc/build_torch_ops.py)."""
-    global _ops
-    if _ops is None:
-        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_grads.so")
-        if not os.path.isfile(path):
-            raise _lib.IncAggLibraryError(
-                f"{path} not found: build it with `python incagg-gnn_amd/csrc/build_torch_ops.py` "
-                "(there is no fallback implementation)")
-        torch.ops.load_library(path)
-        ns = torch.ops.incagg_grads
-        _ops = (ns.grad_norm.default, ns.adam_step_clipped.default)
-    return _ops
-
-
 def _gradients(parameters) -> List[Tensor]:
     if isinstance(parameters, Tensor):
         parameters = (parameters,)
@@ -66,7 +47,7 @@ def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.
     ``inf``."""
     code = _norm_type(norm_type)
     grads = _gradients(parameters)
-    return _grad_ops()[0](grads, code, 0.0, False) if grads else torch.zeros(())
+    return ops.train_ops().grad_norm(grads, code, 0.0, False) if grads else torch.zeros(())
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
@@ -80,7 +61,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     grads = _gradients(parameters)
     if not grads:
         return torch.zeros(())
-    call = _grad_ops()[0]
+    call = ops.train_ops().grad_norm
     if error_if_nonfinite and not bool(torch.isfinite(call(grads, code, 0.0, False))):
         raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is "
                            "non-finite, so it cannot be clipped")
@@ -192,7 +173,7 @@ class Adam:
             live = [k for k, g in enumerate(grads) if g is not None]
             params, states, group_of, grads = ([v[k] for k in live]
                                                for v in (params, states, group_of, grads))
-        return _grad_ops()[1](params, grads, [st["exp_avg"] for st in states],
+        return ops.train_ops().adam_step_clipped(params, grads, [st["exp_avg"] for st in states],
                               [st["exp_avg_sq"] for st in states], [st["step"] for st in states],
                               group_of, hyper, max_norm, self.device)
 
