@@ -1203,7 +1203,12 @@ template <int D> static int launch_rows(GroupedArgs &a, bool trans_w, hipStream_
   const int64_t average = a.rows / a.n_groups;
   if (average <= 16) return launch_rows_tile<D, 16, 64, 1, 4, 2, 4>(a, trans_w, s);
   if (a.n <= 64) return launch_rows_tile<D, 128, 64, 4, 1, STAGES, 1>(a, trans_w, s);
-  if (average <= (F32 ? 768 : 64)) return launch_rows_tile<D, 64, 128, 2, 2, STAGES, 1>(a, trans_w, s);
+  // float32 stays with 64 rows -- more workgroups that take turns between loading, splitting and
+  // multiplying -- until there are a dozen 128 x 128 tiles to a CU (65304 x 256 -> 256 and 16326 x 512
+  // -> 512: 73 / 65 and 82 / 70 us by 128 / 64 rows; 65536 x 1024 -> 1024: 881 / 941)
+  const int64_t large = (int64_t)(a.rows / 128) * ((a.n + 127) / 128);
+  if (average <= (F32 ? 768 : 64) || (F32 && large < 3072))
+    return launch_rows_tile<D, 64, 128, 2, 2, STAGES, 1>(a, trans_w, s);
   if constexpr (!F32) {
     if (pieces(a.x, a.ldx, a.k) && pieces(a.w, a.ldw, trans_w ? a.k : a.n) && a.w_group % 8 == 0) {
       // 256 x 256 halves what a tile reads for its products, but leaves one workgroup to a CU: for
@@ -1271,8 +1276,17 @@ template <int D> static int launch_tn(TnArgs &t, hipStream_t s) {
     if (tn_large_tiles(t.m, t.n, D) && pieces(t.a, t.lda, t.m) && pieces(t.b, t.ldb, t.n))
       return launch_tn_lds<D, 256, 256, 2, 4>(t, s);
   }
-  if (t.m <= 64) return t.n <= 64 ? launch_tn_tile<D, 64, 64>(t, s) : launch_tn_tile<D, 64, 128>(t, s);
-  return t.n <= 64 ? launch_tn_tile<D, 128, 64>(t, s) : launch_tn_tile<D, 128, 128>(t, s);
+  if (t.n <= 64) return t.m <= 64 ? launch_tn_tile<D, 64, 64>(t, s) : launch_tn_tile<D, 128, 64>(t, s);
+  // 128 x 128 tiles load and split less for a product, 64 x 128 leave twice the workgroups to hide
+  // what they wait for.  float32, us by 128 / 64: 16326 rows, 256 x 256 46 / 42, 65304 rows 121 / 112;
+  // 65536 rows, 1024 x 1024 1036 / 1236, 40000 rows in 40 groups, 512 x 512 228 / 244; one column of
+  // tiles, 128064 rows, 256 x 100, 82 / 94.  float16 30000 rows, 300 x 601 174 / 125; bfloat16 30000
+  // rows, 256 x 100 38 / 23.
+  const int64_t tiles = (int64_t)((t.m + 127) / 128) * ((t.n + 127) / 128);
+  if (D == INCAGG_DTYPE_F32 && t.m > 64 &&
+      (t.n <= 128 || (t.rows / t.segment + t.n_groups) * tiles >= 800))
+    return launch_tn_tile<D, 128, 128>(t, s);
+  return launch_tn_tile<D, 64, 128>(t, s);
 }
 
 static int check_groups(const int32_t *ptr, int64_t n_groups, int64_t rows, int dtype) {

@@ -319,6 +319,28 @@ Tensor adam_step_clipped(std::vector<Tensor> params, std::vector<Tensor> grads,
   return scratch.norm;
 }
 
+std::tuple<Tensor, Tensor> group_rows(const Tensor &ids, int64_t n_groups) {
+  TORCH_CHECK(ids.is_cuda(), "ids must live on the GPU: the grouping kernels are HIP only and there "
+              "is no CPU implementation");
+  const bool wide = ids.scalar_type() == at::kLong;
+  TORCH_CHECK_TYPE((wide || ids.scalar_type() == at::kInt) && ids.dim() == 1 && ids.is_contiguous(),
+                   "ids must be a contiguous 1-D int64 or int32 tensor");
+  TORCH_CHECK_VALUE(n_groups >= 1 && n_groups <= incagg_group_rows_max_groups(),
+                    "n_groups must be between 1 and ", incagg_group_rows_max_groups(), ", got ",
+                    n_groups);
+  const int64_t rows = ids.numel(), need = incagg_group_rows_ws_ints(rows, n_groups);
+  check_status(need);
+  const auto options = ids.options().dtype(at::kInt);
+  Tensor order = at::empty({rows}, options), ptr = at::empty({n_groups + 1}, options), ws;
+  if (need) ws = at::empty({need}, options);
+  c10::DeviceGuard guard(ids.device());
+  check_status(incagg_group_rows(
+      ptr_or_null<void>(ids), wide ? 1 : 0, rows, n_groups, need ? ws.data_ptr<int32_t>() : nullptr,
+      need, const_cast<int32_t *>(ptr_or_null<int32_t>(order)), ptr.data_ptr<int32_t>(),
+      current_stream(ids.device())));
+  return {order, ptr};
+}
+
 // ---- the grouped linear layer ------------------------------------------------------------------
 // Rows as the C ABI takes them: unit stride, no two rows in one place (an expanded gradient).
 Tensor plain_rows(const Tensor &t) {
@@ -454,6 +476,7 @@ TORCH_LIBRARY(incagg_train, m) {
   m.def("adam_step_clipped(Tensor[] params, Tensor[] grads, Tensor[] exp_avg, Tensor[] exp_avg_sq, "
         "Tensor[] steps, int[] group, float[] hyper, float max_norm, Device device) -> Tensor",
         &adam_step_clipped);
+  m.def("group_rows(Tensor ids, int n_groups) -> (Tensor, Tensor)", &group_rows);
   m.def("grouped_linear(Tensor x, Tensor weight, Tensor? bias, Tensor ptr, Tensor? order, int n_rows, "
         "int pitch_y, int pitch_dx) -> Tensor", &grouped_linear);
 }

@@ -734,7 +734,8 @@ def softmax_cross_entropy(logits: Tensor, labels: Tensor) -> Tensor:
 
 
 # --------------------------------------------------------------------------- rows of several kinds
-TrainOps = collections.namedtuple("TrainOps", "grad_norm adam_step_clipped grouped_linear")
+TrainOps = collections.namedtuple("TrainOps",
+                                  "grad_norm adam_step_clipped group_rows grouped_linear")
 _train_ops = None
 
 
@@ -796,19 +797,8 @@ def group_rows(ids: Tensor, n_groups: int) -> RowGroups:
     """Rows ordered by the group ``ids[i]`` in ``[0, n_groups)`` each of them belongs to, equal
     ids in row order; ``-1``: the row has no group (incagg_group_rows).  Ids outside
     ``[-1, n_groups)`` are reported by ``check_device_errors``; their rows have no group."""
-    _need_cuda(ids, "ids")
-    _group_index(ids, "ids")
-    n_groups, rows, dev = _max_groups(n_groups), ids.numel(), ids.device
-    L = lib()
-    need = L.incagg_group_rows_ws_ints(rows, n_groups)
-    check(need)
-    order = torch.empty(rows, dtype=torch.int32, device=dev)
-    ptr = torch.empty(n_groups + 1, dtype=torch.int32, device=dev)
-    ws = torch.empty(need, dtype=torch.int32, device=dev) if need else None
-    with _on_device(dev):
-        check(L.incagg_group_rows(_ptr(ids), 1 if ids.dtype == torch.int64 else 0, rows, n_groups,
-                                  _ptr(ws), need, _ptr(order), ptr.data_ptr(), _stream_of(dev)))
-    return RowGroups(order, ptr, rows)
+    order, ptr = train_ops().group_rows(ids, n_groups)
+    return RowGroups(order, ptr, order.shape[0])
 
 
 def groups_from_ptr(ptr: Tensor, n_rows: int) -> RowGroups:

@@ -324,6 +324,30 @@ def test_a_long_reduction_and_many_rows(ops, dev):
                dtype)
 
 
+@pytest.mark.parametrize("dtype,rows,n_groups,k,n", [
+    (BF16, 20_003, 5, 200, 1024),      # large tiles, a ragged last chunk of the reduction
+    (F16, 40_000, 3, 128, 520),        # large tiles, columns that end inside one
+    (BF16, 70_001, 2, 8, 272),         # one chunk, most of it zeros
+    (F16, 33_000, 130, 64, 640),       # more groups than large tiles hold rows for
+    (F32, 100_003, 4, 40, 512),        # the large tiles of float32
+    (BF16, 9_000, 4, 72, 100)])        # 16-byte rows on the one side, not on the other
+def test_large_problems(ops, dev, dtype, rows, n_groups, k, n):
+    gen, x, w, b, dy = _case(dev, rows, n_groups, k, n, dtype, rows + n)
+    for kind in ("ragged", "random"):
+        ids = _ids(kind, rows, n_groups, dev, gen)
+        groups = ops.group_rows(ids, n_groups)
+        _close(ops.grouped_gemm(x, w, groups, trans_w=True, bias=b), *_rows64(x, w, b, ids, True),
+               k + 1, dtype)
+        _close(ops.grouped_gemm(dy, w, groups), *_rows64(dy, w, None, ids, False), n, dtype)
+        wt = w.transpose(1, 2).contiguous()             # the forward product with W given as [k, n]
+        _close(ops.grouped_gemm(x, wt, groups, bias=b), *_rows64(x, wt, b, ids, False), k + 1, dtype)
+        dw, db = ops.grouped_tn(dy, x, groups, column_sums=True)
+        d, mag, s, smag, count = _tn64(dy, x, ids, n_groups)
+        _close(dw, d, mag, count.view(-1, 1, 1), dtype)
+        _close(db, s, smag, count.view(-1, 1), dtype)
+        assert torch.equal(ops.grouped_tn(dy, x, groups), dw)
+
+
 def test_no_rows(ops, dev):
     groups = ops.group_rows(torch.empty(0, dtype=torch.int64, device=dev), 3)
     w = torch.randn(3, 5, 4, device=dev)
