@@ -112,9 +112,27 @@ __device__ inline void put_split(unsigned short *tile, int at, const float (&v)[
   *reinterpret_cast<u4 *>(tile + 2 * PLANE + at) = l;
 }
 
-// Rows whose k values are contiguous: ROWS x BK, a thread takes U pieces of 8 values.  The loads
-// of a whole chunk have no condition in them (a branch per piece would make each wait for the one
-// before).
+// 16 bytes shifted down by `bits` (0 .. 128), zeros behind.
+__device__ inline Pack<unsigned, 4> shift_down(Pack<unsigned, 4> v, int bits) {
+  typedef unsigned long long u64;
+  u64 lo = v.v[0] | (u64)v.v[1] << 32, hi = v.v[2] | (u64)v.v[3] << 32;
+  if (bits >= 64) {
+    lo = hi;
+    hi = 0;
+    bits -= 64;
+  }
+  if (bits >= 64) lo = 0;
+  else if (bits > 0) {
+    lo = lo >> bits | hi << (64 - bits);
+    hi >>= bits;
+  }
+  return {{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)}};
+}
+
+// Loads at ragged edges are whole vectors as well, of what lies in front of the edge, shifted: a
+// load per element under a condition of its own would wait for the one before it.
+
+// Rows whose k values are contiguous: ROWS x BK, a thread takes U pieces of 8 values.
 template <int D, int ROWS, int THREADS> struct RowStage {
   typedef typename Type<D>::Raw Raw;
   static constexpr int BK = Type<D>::BK, CH = BK / 8, UNITS = ROWS * CH;
@@ -135,25 +153,30 @@ template <int D, int ROWS, int THREADS> struct RowStage {
       r[i] = __builtin_bit_cast(Pack<unsigned, W>,
                                 *reinterpret_cast<const Pack<Raw, 8> *>(src[i] + k0));
   }
+  // the last chunk of a row of k values
   __device__ void load_tail(int k0, int k) {
+    constexpr int N = 16 / sizeof(Raw);
 #pragma unroll
     for (int i = 0; i < U; i++) {
-      const int left = k - k0 - (unit(i) % CH) * 8;
-      constexpr int N = 16 / sizeof(Raw);
-      Pack<Raw, 8> v;
+      const int at = (unit(i) % CH) * 8;
+      const Raw *row = src[i] - at;
 #pragma unroll
       for (int h = 0; h < 8; h += N) {
-        Pack<Raw, N> q;
-        if (left >= h + N) {
-          q = *reinterpret_cast<const Pack<Raw, N> *>(src[i] + k0 + h);
+        const int left = k - k0 - at - h;           // values from here to the row's end
+        Pack<unsigned, 4> q;
+        if (k >= N) {
+          q = *reinterpret_cast<const Pack<unsigned, 4> *>(
+              reinterpret_cast<const Pack<Raw, N> *>(row + (left >= N ? k0 + at + h : k - N)));
+          q = shift_down(q, (N - min(max(left, 0), N)) * 8 * (int)sizeof(Raw));
         } else {
+          Pack<Raw, N> v;
 #pragma unroll
-          for (int e = 0; e < N; e++) q.v[e] = h + e < left ? src[i][k0 + h + e] : (Raw)0;
+          for (int e = 0; e < N; e++) v.v[e] = e < left ? row[k0 + at + h + e] : (Raw)0;
+          q = __builtin_bit_cast(Pack<unsigned, 4>, v);
         }
 #pragma unroll
-        for (int e = 0; e < N; e++) v.v[h + e] = q.v[e];
+        for (int e = 0; e < 4; e++) r[i].v[h * (int)sizeof(Raw) / 4 + e] = q.v[e];
       }
-      r[i] = __builtin_bit_cast(Pack<unsigned, W>, v);
     }
   }
   __device__ void store(unsigned short *tile) {
@@ -172,64 +195,81 @@ template <int D, int ROWS, int THREADS> struct RowStage {
   }
 };
 
-// The transposing form: rows along the reduction, COLS columns of them become the tile's rows.  A
-// thread takes 8 rows x V columns.
+// The transposing form: rows along the reduction, COLS columns of them (from `first` of a matrix of n
+// on) become the tile's rows.  A thread takes 8 rows x V columns.
 template <int D, int COLS, int THREADS> struct ColStage {
   typedef typename Type<D>::Raw Raw;
-  static constexpr int BK = Type<D>::BK;
-  static constexpr int V = COLS * BK / 8 >= THREADS ? COLS * BK / 8 / THREADS : 1;
-  static constexpr int GROUPS = COLS / V;
-  Pack<Raw, V> r[8];
+  static constexpr int BK = Type<D>::BK, V = COLS * BK / 8 / THREADS, GROUPS = COLS / V;
+  static_assert(V >= 1 && V <= 4 && GROUPS * (BK / 8) == THREADS, "every thread takes 8 x V values");
+  typedef Raw Row __attribute__((ext_vector_type(V)));
+  Row r[8];
+  int at, shift, cols;                  // where this thread's columns are loaded from, moved by what
+  bool narrow;                          // a matrix of fewer columns than a vector has
   static __device__ int col() { return ((int)threadIdx.x % GROUPS) * V; }
   static __device__ int row() { return ((int)threadIdx.x / GROUPS) * 8; }
-  static __device__ bool active() { return GROUPS * (BK / 8) >= THREADS || row() < BK; }
-  // row i (0 .. 7) of this thread starts at row_of(i)
-  template <typename F> __device__ void load(F &&row_of) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) r[i] = *reinterpret_cast<const Pack<Raw, V> *>(row_of(i));
+  __device__ void init(int first, int n) {
+    narrow = n < V;
+    cols = n - first - col();
+    at = narrow ? first + col() : min(first + col(), n - V);
+    shift = narrow || cols <= 0 ? 0 : first + col() - at;   // (columns behind the last: dropped)
   }
-  // the same with rows that are not there (NULL); `cols`: columns from this thread's first one to
-  // the matrix's end
-  template <typename F> __device__ void load_tail(int cols, F &&row_of) {
+  // row i (0 .. 7) of this thread starts at row_of(i), which has to be a row of the matrix
+  template <typename F> __device__ void load(F &&row_of) {
+    if (!narrow) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const Raw *p = row_of(i);
-      if (p && cols >= V) {
-        r[i] = *reinterpret_cast<const Pack<Raw, V> *>(p);
-      } else {
+      for (int i = 0; i < 8; i++)
+        r[i] = __builtin_bit_cast(Row, *reinterpret_cast<const Pack<Raw, V> *>(row_of(i) + at));
+    } else {
 #pragma unroll
-        for (int e = 0; e < V; e++) r[i].v[e] = p && e < cols ? p[e] : (Raw)0;
+      for (int i = 0; i < 8; i++) {
+        const Raw *p = row_of(i) + at;
+#pragma unroll
+        for (int e = 0; e < V; e++) r[i][e] = e < cols ? p[e] : (Raw)0;
       }
     }
   }
-  // The thread's first column, of a matrix of n, when its columns end where vectors do: columns
-  // behind the last repeat the last vector (their results are dropped).
-  static __device__ bool whole_vectors(int first, int n) { return first + COLS <= n || (n >= V && n % V == 0); }
-  static __device__ int col_within(int first, int n) { return first + COLS <= n ? first + col() : min(first + col(), n - V); }
+  // rows from `count` on are not part of the reduction
+  __device__ void clear_from(int count) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) clear_row(i, i < count);
+  }
   __device__ void clear_row(int i, bool keep) {
 #pragma unroll
-    for (int e = 0; e < V; e++) r[i].v[e] = keep ? r[i].v[e] : (Raw)0;
+    for (int e = 0; e < V; e++) r[i][e] = keep ? r[i][e] : (Raw)0;
+  }
+  // moves the columns of the edge's thread to where they belong (once, in front of store)
+  __device__ void settle() {
+    if (V == 1 || shift == 0) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        Raw v = (Raw)0;
+#pragma unroll
+        for (int f = e + 1; f < V; f++) v = f - e == shift ? r[i][f] : v;
+        r[i][e] = v;
+      }
   }
   __device__ void store(unsigned short *tile) {
-    if (!active()) return;
 #pragma unroll
     for (int e = 0; e < V; e++) {
       const int at = piece_at<BK>(col() + e, row() / 8);
       if constexpr (D == INCAGG_DTYPE_F32) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = r[i].v[e];
+        for (int i = 0; i < 8; i++) v[i] = r[i][e];
         put_split<COLS * BK>(tile, at, v);
       } else {
         u4 h;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           if constexpr (V >= 2) {       // halves of two dwords into one
-            const unsigned lo = __builtin_bit_cast(Pack<unsigned, V / 2>, r[2 * i]).v[e / 2];
-            const unsigned hi = __builtin_bit_cast(Pack<unsigned, V / 2>, r[2 * i + 1]).v[e / 2];
+            typedef unsigned Pairs __attribute__((ext_vector_type(V / 2)));
+            const unsigned lo = __builtin_bit_cast(Pairs, r[2 * i])[e / 2];
+            const unsigned hi = __builtin_bit_cast(Pairs, r[2 * i + 1])[e / 2];
             h[i] = __builtin_amdgcn_perm(hi, lo, e & 1 ? 0x07060302u : 0x05040100u);
           } else {
-            h[i] = (unsigned)r[2 * i].v[e] | ((unsigned)r[2 * i + 1].v[e] << 16);
+            h[i] = (unsigned)r[2 * i][e] | ((unsigned)r[2 * i + 1][e] << 16);
           }
         }
         *reinterpret_cast<u4 *>(tile + at) = h;
@@ -467,7 +507,8 @@ template <int D> struct RowsOut {
 
 // ---- Y = X W + b -----------------------------------------------------------------------------------
 template <int D, int BM, int BN, int WM, int WN, bool TRANS_W, int STAGES, int FLIGHT>
-__global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_kernel(const GroupedArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, BM == 64 && D == INCAGG_DTYPE_F32 ? 4 : 2)
+void grouped_rows_kernel(const GroupedArgs a) {
   typedef typename Type<D>::Raw Raw;
   constexpr int T = 64 * WM * WN, BK = Type<D>::BK, P = Type<D>::P;
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
@@ -491,27 +532,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_kernel(const Gro
     // (rows and columns outside the matrices repeat one inside; their results are dropped)
     RowStage<D, BM, T> xs[FLIGHT];
     RowStage<D, TRANS_W ? BN : 16, T> wr[FLIGHT];
-    ColStage<D, TRANS_W ? 16 : BN, T> wc[FLIGHT];
+    ColStage<D, TRANS_W ? T * 8 / BK : BN, T> wc[FLIGHT];
     if constexpr (TRANS_W)
 #pragma unroll
       for (int f = 0; f < FLIGHT; f++)
         wr[f].init([&](int c) { return w + (long long)min(n0 + c, a.n - 1) * a.ldw; });
     const int n_chunks = (a.k + BK - 1) / BK;
-    const bool whole_cols = wc[0].whole_vectors(n0, a.n);
+    if constexpr (!TRANS_W)
+#pragma unroll
+      for (int f = 0; f < FLIGHT; f++) wc[f].init(n0, a.n);
     auto load_w = [&](int c, int f) __attribute__((always_inline)) {
       const int k0 = c * BK;
-      const bool whole = k0 + BK <= a.k;
       if constexpr (TRANS_W) {
-        if (whole) wr[f].load(k0);
+        if (k0 + BK <= a.k) wr[f].load(k0);
         else wr[f].load_tail(k0, a.k);
       } else {
         const int r0 = k0 + wc[f].row();
-        const int n = whole_cols ? wc[f].col_within(n0, a.n) : n0 + wc[f].col();
-        const Raw *p = w + (long long)r0 * a.ldw + n;
-        if (whole && whole_cols && wc[f].active())
+        if (k0 + BK <= a.k) {
+          const Raw *p = w + (long long)r0 * a.ldw;
           wc[f].load([&](int i) { return p + i * a.ldw; });
-        else
-          wc[f].load_tail(a.n - n, [&](int i) { return r0 + i < a.k ? p + i * a.ldw : nullptr; });
+        } else {
+          wc[f].load([&](int i) { return w + (long long)min(r0 + i, a.k - 1) * a.ldw; });
+          wc[f].clear_from(a.k - r0);
+        }
       }
     };
     auto load_x = [&](int c, int f) __attribute__((always_inline)) {
@@ -524,8 +567,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_rows_kernel(const Gro
     };
     auto store = [&](int s, int f) __attribute__((always_inline)) {
       xs[f].store(xt + s * P * BM * BK);
-      if constexpr (TRANS_W) wr[f].store(wt + s * P * BN * BK);
-      else wc[f].store(wt + s * P * BN * BK);
+      if constexpr (TRANS_W) {
+        wr[f].store(wt + s * P * BN * BK);
+      } else {
+        wc[f].settle();
+        wc[f].store(wt + s * P * BN * BK);
+      }
     };
     // (the first weights are on their way while the row numbers arrive, which the rows wait for)
 #pragma unroll
@@ -666,56 +713,55 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
   ColStage<D, BM, T> as;
   ColStage<D, BN, T> bs;
   float sums[decltype(as)::V] = {};
-  const int acols = t.m - m0 - as.col(), bcols = t.n - n0 - bs.col();
+  // (copies: captured as members of the argument, they would be read from memory in the loop)
+  const int *const order = t.order;
+  const long long lda = t.lda, ldb = t.ldb;
+  const unsigned last_row = t.rows - 1u;
+  as.init(m0, t.m);
+  bs.init(n0, t.n);
   // row numbers of a chunk are fetched one chunk ahead of its rows
-  const bool whole_a = as.whole_vectors(m0, t.m), whole_b = bs.whole_vectors(n0, t.n);
-  const Raw *const pa = a + (whole_a ? as.col_within(m0, t.m) : m0 + as.col());
-  const Raw *const pb = b + (whole_b ? bs.col_within(n0, t.n) : n0 + bs.col());
-  Pack<int, 8> ia, ib;
-  auto fetch_ids = [&](int r0) {
-    if (!t.order) return;
+  typedef int Ids __attribute__((ext_vector_type(8)));
+  Ids ia, ib;
+  auto fetch_ids = [&](int r0) __attribute__((always_inline)) {
+    if (!order) return;
     if (r0 + BK <= last) {
-      ia = *reinterpret_cast<const Pack<int, 8> *>(t.order + r0 + min(as.row(), BK - 8));
-      ib = *reinterpret_cast<const Pack<int, 8> *>(t.order + r0 + min(bs.row(), BK - 8));
+      ia = __builtin_bit_cast(Ids, *reinterpret_cast<const Pack<int, 8> *>(order + r0 + as.row()));
+      ib = __builtin_bit_cast(Ids, *reinterpret_cast<const Pack<int, 8> *>(order + r0 + bs.row()));
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        ia.v[i] = t.order[min(r0 + as.row() + i, last - 1)];
-        ib.v[i] = t.order[min(r0 + bs.row() + i, last - 1)];
+        ia[i] = order[min(r0 + as.row() + i, last - 1)];
+        ib[i] = order[min(r0 + bs.row() + i, last - 1)];
       }
     }
   };
-  auto load = [&](int r0) {
+  auto load = [&](int r0) __attribute__((always_inline)) {
     const int ra = r0 + as.row(), rb = r0 + bs.row();
-    // (only rows inside the matrices are named)
-    auto row_a = [&](int i) {
-      return pa + (long long)(t.order ? min((unsigned)ia.v[i], (unsigned)t.rows - 1u) : ra + i) * t.lda;
-    };
-    auto row_b = [&](int i) {
-      return pb + (long long)(t.order ? min((unsigned)ib.v[i], (unsigned)t.rows - 1u) : rb + i) * t.ldb;
-    };
-    const bool whole_rows = r0 + BK <= last;
-    if (whole_rows && whole_a && as.active()) as.load(row_a);
-    else
-      as.load_tail(whole_a ? BM : acols, [&](int i) -> const Raw * {
-        return ra + i < last && as.active() ? row_a(i) : nullptr;
-      });
-    if (whole_rows && whole_b && bs.active()) bs.load(row_b);
-    else
-      bs.load_tail(whole_b ? BN : bcols, [&](int i) -> const Raw * {
-        return rb + i < last && bs.active() ? row_b(i) : nullptr;
-      });
-    if (t.order) {      // rows of no matrix: zeros, and reported
+    // (rows behind the last repeat it, row numbers outside the matrix its last row: cleared below)
+    if (order) {
+      as.load([&](int i) { return a + (long long)min((unsigned)ia[i], last_row) * lda; });
+      bs.load([&](int i) { return b + (long long)min((unsigned)ib[i], last_row) * ldb; });
+    } else {
+      const int la = last - 1 - ra, lb = last - 1 - rb;
+      const Raw *pa = a + (long long)min(ra, last - 1) * lda, *pb = b + (long long)min(rb, last - 1) * ldb;
+      as.load([&](int i) { return i <= la ? pa + i * lda : pa; });
+      bs.load([&](int i) { return i <= lb ? pb + i * ldb : pb; });
+    }
+    if (r0 + BK > last) {
+      as.clear_from(last - ra);
+      bs.clear_from(last - rb);
+    }
+    if (order) {      // rows of no matrix: zeros, and reported
       bool bad = false;
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        bad |= (unsigned)ia.v[i] >= (unsigned)t.rows || (unsigned)ib.v[i] >= (unsigned)t.rows;
+        bad |= (unsigned)ia[i] > last_row || (unsigned)ib[i] > last_row;
       if (bad) {
         *t.err = 1;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          as.clear_row(i, (unsigned)ia.v[i] < (unsigned)t.rows);
-          bs.clear_row(i, (unsigned)ib.v[i] < (unsigned)t.rows);
+          as.clear_row(i, (unsigned)ia[i] <= last_row);
+          bs.clear_row(i, (unsigned)ib[i] <= last_row);
         }
       }
     }
@@ -726,14 +772,16 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
     load(first);
     for (int r0 = first; r0 < last; r0 += BK) {
       if (r0 > first) __syncthreads();
+      as.settle();
+      bs.settle();
       as.store(at);
       bs.store(bt);
-      if (want_sums && as.active())
+      if (want_sums)
 #pragma unroll
         for (int e = 0; e < decltype(as)::V; e++) {
           float s = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; i++) s += raw_to_float<D>(as.r[i].v[e]);
+          for (int i = 0; i < 8; i++) s += raw_to_float<D>(as.r[i][e]);
           sums[e] += s;
         }
       __syncthreads();
@@ -770,9 +818,8 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
   static_assert(sizeof(float) * RG * BM <= sizeof(tiles), "reduction space");
   float *red = reinterpret_cast<float *>(tiles);
   __syncthreads();
-  if (as.active())
 #pragma unroll
-    for (int e = 0; e < V; e++) red[(as.row() / 8) * BM + as.col() + e] = sums[e];
+  for (int e = 0; e < V; e++) red[(as.row() / 8) * BM + as.col() + e] = sums[e];
   __syncthreads();
   for (int c = tid; c < BM && m0 + c < t.m; c += T) {
     float s = 0.f;
@@ -1207,7 +1254,7 @@ template <int D> static int launch_rows(GroupedArgs &a, bool trans_w, hipStream_
   // multiplying -- until there are a dozen 128 x 128 tiles to a CU (65304 x 256 -> 256 and 16326 x 512
   // -> 512: 73 / 65 and 82 / 70 us by 128 / 64 rows; 65536 x 1024 -> 1024: 881 / 941)
   const int64_t large = (int64_t)(a.rows / 128) * ((a.n + 127) / 128);
-  if (average <= (F32 ? 768 : 64) || (F32 && large < 3072))
+  if (average <= (F32 ? 768 : 64) || (F32 && large < 3000))
     return launch_rows_tile<D, 64, 128, 2, 2, STAGES, 1>(a, trans_w, s);
   if constexpr (!F32) {
     if (pieces(a.x, a.ldx, a.k) && pieces(a.w, a.ldw, trans_w ? a.k : a.n) && a.w_group % 8 == 0) {
@@ -1282,10 +1329,11 @@ template <int D> static int launch_tn(TnArgs &t, hipStream_t s) {
   // 65536 rows, 1024 x 1024 1036 / 1236, 40000 rows in 40 groups, 512 x 512 228 / 244; one column of
   // tiles, 128064 rows, 256 x 100, 82 / 94.  float16 30000 rows, 300 x 601 174 / 125; bfloat16 30000
   // rows, 256 x 100 38 / 23.
-  const int64_t tiles = (int64_t)((t.m + 127) / 128) * ((t.n + 127) / 128);
-  if (D == INCAGG_DTYPE_F32 && t.m > 64 &&
-      (t.n <= 128 || (t.rows / t.segment + t.n_groups) * tiles >= 800))
-    return launch_tn_tile<D, 128, 128>(t, s);
+  if constexpr (D == INCAGG_DTYPE_F32) {
+    const int64_t tiles = (int64_t)((t.m + 127) / 128) * ((t.n + 127) / 128);
+    if (t.m > 64 && (t.n <= 128 || (t.rows / t.segment + t.n_groups) * tiles >= 800))
+      return launch_tn_tile<D, 128, 128>(t, s);
+  }
   return launch_tn_tile<D, 64, 128>(t, s);
 }
 
