@@ -533,7 +533,7 @@ static int adam_clip_call(const incagg_adam_clip_segment *segs, int64_t n_segs,
       t.hyper[k] = (unsigned char)h;
       t.first_block[k] = (int)blocks;
       blocks += (a.n + per_block - 1) / per_block;
-      INCAGG_REQUIRE(blocks < (1ll << 30), "grid too large");
+      INCAGG_REQUIRE(blocks < (1ll << 24), "grid too large");      // (2^32 threads a launch)
     }
     t.first_block[k] = (int)blocks;
     t.n_segs = k;

@@ -703,7 +703,7 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
   if (g >= t.n_groups || seg < 0 || (!any && seg > 0)) return;
   const int begin = group_begin(t.ptr, g, t.rows);
   const bool whole = end - begin <= t.segment;       // the group's only segment (or an empty group)
-  const int last = min(end, first + t.segment);
+  const int last = first + min(end - first, t.segment);      // (first + segment may pass 2^31)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row0 = (wave >> 1) * (BM / 2), col0 = (wave & 1) * (BN / 2);
   const Raw *a = static_cast<const Raw *>(t.a), *b = static_cast<const Raw *>(t.b);
@@ -1070,7 +1070,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_tn_lds_kernel(const T
   g = __builtin_amdgcn_readfirstlane(g);
   const int begin = group_begin(t.ptr, g, t.rows);
   const bool whole = end - begin <= t.segment;       // the group's only segment (or an empty group)
-  const int last = __builtin_amdgcn_readfirstlane(min(end, first + t.segment));
+  const int last = __builtin_amdgcn_readfirstlane(first + min(end - first, t.segment));
   first = __builtin_amdgcn_readfirstlane(first);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int row0 = (wave / WN) * (BM / WM), col0 = (wave % WN) * (BN / WN);
@@ -1201,11 +1201,13 @@ template <int D> __global__ __launch_bounds__(256) void grouped_tn_finish_kernel
 }
 
 // ---- host side ---------------------------------------------------------------------------------------
+constexpr int64_t kMaxThreads = 1ll << 32;       // of a launch
+
 template <int D, int BM, int BN, int WM, int WN, int STAGES, int FLIGHT>
 static int launch_rows_tile(GroupedArgs &a, bool trans_w, hipStream_t s) {
   a.n_tiles = (a.n + BN - 1) / BN;
   const int64_t blocks = ((int64_t)a.rows / BM + a.n_groups + 1) * a.n_tiles;
-  INCAGG_REQUIRE(blocks < (1ll << 31), "too many rows and columns for one call");
+  INCAGG_REQUIRE(blocks * (64 * WM * WN) < kMaxThreads, "too many rows and columns for one call");
   const dim3 grid((unsigned)blocks), block(64 * WM * WN);
   if (trans_w)
     hipLaunchKernelGGL((grouped_rows_kernel<D, BM, BN, WM, WN, true, STAGES, FLIGHT>), grid, block, 0, s, a);
@@ -1219,7 +1221,7 @@ template <int D, int BM, int BN, int WM, int WN>
 static int launch_rows_lds(GroupedArgs &a, bool trans_w, hipStream_t s) {
   a.n_tiles = (a.n + BN - 1) / BN;
   const int64_t blocks = ((int64_t)a.rows / BM + a.n_groups + 1) * a.n_tiles;
-  INCAGG_REQUIRE(blocks < (1ll << 31), "too many rows and columns for one call");
+  INCAGG_REQUIRE(blocks * (64 * WM * WN) < kMaxThreads, "too many rows and columns for one call");
   const dim3 grid((unsigned)blocks), block(64 * WM * WN);
   if (trans_w)
     hipLaunchKernelGGL((grouped_rows_lds_kernel<D, BM, BN, WM, WN, true>), grid, block, 0, s, a);
@@ -1300,7 +1302,7 @@ template <int D, int BM, int BN> static int launch_tn_tile(TnArgs &t, hipStream_
   t.m_tiles = (t.m + BM - 1) / BM;
   t.n_tiles = (t.n + BN - 1) / BN;
   const int64_t blocks = ((int64_t)t.rows / t.segment + t.n_groups) * t.m_tiles * t.n_tiles;
-  INCAGG_REQUIRE(blocks < (1ll << 31), "too many rows and columns for one call");
+  INCAGG_REQUIRE(blocks * 256 < kMaxThreads, "too many rows and columns for one call");
   hipLaunchKernelGGL((grouped_tn_kernel<D, BM, BN>), dim3((unsigned)blocks), dim3(256), 0, s, t);
   INCAGG_HIP_TRY(hipGetLastError());
   return tn_finish<D>(t, s);
@@ -1311,7 +1313,7 @@ static int launch_tn_lds(TnArgs &t, hipStream_t s) {
   t.m_tiles = (t.m + BM - 1) / BM;
   t.n_tiles = (t.n + BN - 1) / BN;
   const int64_t blocks = ((int64_t)t.rows / t.segment + t.n_groups) * t.m_tiles * t.n_tiles;
-  INCAGG_REQUIRE(blocks < (1ll << 31), "too many rows and columns for one call");
+  INCAGG_REQUIRE(blocks * (64 * WM * WN) < kMaxThreads, "too many rows and columns for one call");
   hipLaunchKernelGGL((grouped_tn_lds_kernel<D, BM, BN, WM, WN>), dim3((unsigned)blocks),
                      dim3(64 * WM * WN), 0, s, t);
   INCAGG_HIP_TRY(hipGetLastError());

@@ -16,8 +16,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 #ifdef INCAGG_OPS_TRAIN
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #endif
 
 #include <deque>
@@ -208,8 +210,9 @@ int64_t element_code(const Tensor &t) {
   }
 }
 
-// The gradients as segments; those that are not contiguous as copies (`dense`), which are written
-// back behind the call when `scaled`.
+// The gradients as segments.  What is wanted of them does not depend on the order of their elements,
+// so a transposed one is taken as it lies; those with gaps go in as copies (`dense`), which are
+// written back behind the call when `scaled`.
 struct Segments {
   std::vector<incagg_norm_segment> segs;
   std::vector<std::pair<size_t, Tensor>> dense;
@@ -226,10 +229,14 @@ struct Segments {
                        g.scalar_type());
       TORCH_CHECK_VALUE(g.device() == grads[0].device(), "all gradients must be on one device");
       void *p = g.numel() ? g.data_ptr() : nullptr;
-      if (!g.is_contiguous()) {
-        if (scaled && g.numel() > 1)
-          for (int64_t st : g.strides())
-            TORCH_CHECK(st != 0, "a gradient's elements overlap in memory (an expanded tensor)");
+      if (!g.unsafeGetTensorImpl()->is_non_overlapping_and_dense()) {
+        if (scaled) {
+          if (g.numel() > 1)
+            for (int64_t st : g.strides())
+              TORCH_CHECK(st != 0, "a gradient's elements overlap in memory (an expanded tensor)");
+          for (const auto &d : dense)           // (the others' memory is compared by the call itself)
+            TORCH_CHECK(grads[d.first].data_ptr() != p, "two gradients overlap in memory");
+        }
         dense.emplace_back(i, g.detach().contiguous());
         p = dense.back().second.data_ptr();
       }
@@ -404,6 +411,19 @@ std::pair<Tensor, Tensor> grouped_tn(const Tensor &a_in, const Tensor &b_in, con
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// A backward pass that is recorded into a HIP graph must not meet a leaf whose accumulation node a
+// graph of the default stream keeps alive: autograd would tie the recording to that stream, which
+// ends the process.  An error instead, before anything of it runs.
+void check_recording(const Tensor &leaf) {
+  if (!leaf.requires_grad() || !leaf.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (!node) return;
+  const auto stream = node->stream();
+  TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(leaf.device().index()).id(),
+              "recording a backward pass while an earlier, eager graph of the same leaf is alive "
+              "(a loss or output that is still referenced): delete it before the recording begins");
+}
+
 struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w,
                         const std::optional<Tensor> &bias, const Tensor &ptr,
@@ -422,6 +442,13 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
     const bool has_bias = ctx->saved_data["bias"].toBool();
     const bool need_w = ctx->needs_input_grad(1), need_b = has_bias && ctx->needs_input_grad(2);
     variable_list out(7);
+    {
+      c10::DeviceGuard guard(x.device());
+      if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+        check_recording(x);
+        check_recording(w);
+      }
+    }
     {
       at::AutoGradMode no_graph(false);
       if (ctx->needs_input_grad(0))

@@ -761,14 +761,23 @@ DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # INC
 class RowGroups:
     """Which rows belong to which group (node type, expert, partition): ``order`` (int32 [rows];
     ``None``: the rows lie sorted already) lists the row numbers group by group, rows of no group
-    last; group ``g`` is ``order[ptr[g]:ptr[g + 1]]`` (int32 [n_groups + 1]).  A pure function of
-    the rows' kinds, built by :func:`group_rows` or :func:`groups_from_ptr` once per batch and
-    passed to every grouped product over those rows.  The sizes of the groups stay on the GPU:
-    nothing here waits for it."""
+    last, each once; group ``g`` is ``order[ptr[g]:ptr[g + 1]]`` (int32 [n_groups + 1]).  A pure
+    function of the rows' kinds, built by :func:`group_rows` or :func:`groups_from_ptr` once per
+    batch and passed to every grouped product over those rows.  The sizes of the groups stay on the
+    GPU: nothing here waits for it."""
 
     def __init__(self, order: Optional[Tensor], ptr: Tensor, n_rows: int):
-        self.order, self.ptr, self.n_rows = order, ptr, int(n_rows)
-        self.n_groups = ptr.numel() - 1
+        self._set(order, ptr, int(n_rows))
+        for t, size, name in ((ptr, self.n_groups + 1, "ptr"), (order, self.n_rows, "order")):
+            if t is not None and (t.dtype != torch.int32 or t.shape != (size,)
+                                  or not t.is_contiguous() or t.device != ptr.device):
+                raise ValueError(f"{name} must be a contiguous int32 [{size}] tensor on the device "
+                                 f"of ptr, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        _max_groups(self.n_groups)
+
+    def _set(self, order, ptr, n_rows):
+        self.order, self.ptr, self.n_rows, self.n_groups = order, ptr, n_rows, ptr.shape[-1] - 1
+        return self
 
     @property
     def device(self):
@@ -798,7 +807,7 @@ def group_rows(ids: Tensor, n_groups: int) -> RowGroups:
     ids in row order; ``-1``: the row has no group (incagg_group_rows).  Ids outside
     ``[-1, n_groups)`` are reported by ``check_device_errors``; their rows have no group."""
     order, ptr = train_ops().group_rows(ids, n_groups)
-    return RowGroups(order, ptr, order.shape[0])
+    return RowGroups.__new__(RowGroups)._set(order, ptr, order.shape[0])
 
 
 def groups_from_ptr(ptr: Tensor, n_rows: int) -> RowGroups:
@@ -842,6 +851,22 @@ def _plain_rows(t: Tensor) -> Tensor:
     return t
 
 
+def _rows_meet(a: Tensor, b: Tensor) -> bool:
+    """Whether two matrices of unit-stride rows may share memory (other columns of the same wider
+    rows do not)."""
+    size, first = a.element_size(), (b.data_ptr() - a.data_ptr())
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    end_a = (a.shape[0] - 1) * _ld(a) + a.shape[1]
+    end_b = (b.shape[0] - 1) * _ld(b) + b.shape[1]
+    if first >= end_a * size or -first >= end_b * size:
+        return False
+    if _ld(a) != _ld(b) or first % size or a.shape[0] < 2 or b.shape[0] < 2:
+        return True
+    at = first // size % _ld(a)
+    return at < a.shape[1] or at + b.shape[1] > _ld(a)
+
+
 def grouped_gemm(x: Tensor, w: Tensor, groups: RowGroups, trans_w: bool = False,
                  bias: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
     """``y[i] = x[i] @ W[g] + bias[g]`` with ``g`` the group of row ``i`` (incagg_grouped_gemm);
@@ -879,6 +904,10 @@ def grouped_gemm(x: Tensor, w: Tensor, groups: RowGroups, trans_w: bool = False,
         _grouped_rows(out, "out", groups, dt)
         if out.shape[1] != n or _plain_rows(out) is not out:
             raise ValueError(f"out must be [{rows}, {n}] with unit-stride rows")
+        span = (n_groups - 1) * w_group + (w.shape[1] - 1) * ldw + w.shape[2]    # from w's first value
+        if (_rows_meet(out, x) or _rows_meet(out, w.as_strided((1, span), (span, 1)))
+                or (bias is not None and _rows_meet(out, bias))):
+            raise RuntimeError("out must not alias an operand: they overlap in memory")
     with _on_device(dev):
         check(lib().incagg_grouped_gemm(
             _ptr(x), _ld(x), w.data_ptr(), ldw, w_group, 1 if trans_w else 0, _ptr(bias), ld_bias,

@@ -183,6 +183,28 @@ def test_refusals(optim, dev):
         optim.grad_norm([d])
 
 
+def test_gradients_with_gaps_and_transposed_ones(optim, dev):
+    """A transposed gradient is scaled where it lies; columns of a wider matrix keep their
+    neighbours; the same columns listed twice are refused."""
+    gen = torch.Generator(device=dev).manual_seed(9)
+    wide = torch.randn(50, 40, device=dev, generator=gen)
+    flip = torch.randn(30, 20, device=dev, generator=gen)
+    params = [torch.nn.Parameter(torch.empty(50, 15, device=dev)) for _ in range(2)]
+    params.append(torch.nn.Parameter(torch.empty(20, 30, device=dev)))
+    params[0].grad, params[1].grad, params[2].grad = wide[:, 3:18], wide[:, 18:33], flip.t()
+    before, guard = [p.grad.clone() for p in params], wide.clone()
+    want = _norm64(before, 2.0)
+    got = optim.clip_grad_norm_(params, 0.25 * want)
+    assert abs(float(got) - want) <= 2.0 ** -23 * want
+    _check_clipped(before, [p.grad for p in params], 0.25 * want / (want + 1e-6))
+    assert torch.equal(wide[:, :3], guard[:, :3]) and torch.equal(wide[:, 33:], guard[:, 33:])
+    params[1].grad = params[0].grad
+    kept = wide.clone()
+    with pytest.raises(RuntimeError, match="overlap"):
+        optim.clip_grad_norm_(params, 0.1)
+    assert torch.equal(wide, kept)
+
+
 # ------------------------------------------------------------------ Adam
 def _adam64(p, g, m, v, t, coef, lr, b1, b2, eps, wd):
     d = g * coef + wd * p

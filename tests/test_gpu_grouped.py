@@ -384,6 +384,75 @@ def test_offsets_past_32_bits(ops, dev):
 
 
 # ------------------------------------------------------------------ the layer
+def test_a_last_row_near_the_limit(ops, dev):
+    """The segments of a sum over nearly 2^31 rows end at the last row (not at a sum that passed
+    2^31)."""
+    rows = 2 ** 31 - 5000
+    a, b = (torch.zeros(rows, 1, device=dev, dtype=BF16) for _ in range(2))
+    a[-5:] = 1.0
+    b[-5:] = 3.0
+    ptr = torch.tensor([0, rows - 300, rows], device=dev)
+    d, sums = ops.grouped_tn(a, b, ops.groups_from_ptr(ptr, rows), column_sums=True)
+    assert d.flatten().tolist() == [0.0, 15.0] and sums.flatten().tolist() == [0.0, 5.0]
+
+
+def test_out_may_lie_beside_an_operand_but_not_over_it(ops, dev):
+    gen, x, w, bias, dy = _case(dev, 300, 3, 24, 24, F32, 7)
+    groups = ops.group_rows(_ids("random", 300, 3, dev, gen), 3)
+    want = ops.grouped_gemm(x, w, groups, trans_w=True)
+    wide = torch.zeros(300, 60, device=dev)
+    wide[:, 10:34] = x
+    got = ops.grouped_gemm(wide[:, 10:34], w, groups, trans_w=True, out=wide[:, 34:58])
+    assert torch.equal(got, want) and torch.equal(wide[:, 10:34], x)
+    assert float(wide[:, :10].abs().sum()) == 0.0 and float(wide[:, 58:].abs().sum()) == 0.0
+    flat = torch.randn(40_000, device=dev, generator=gen)
+    rows = flat[:7200].view(300, 24)
+    for over in (wide[:, 11:35], wide[:, 33:57], wide[:, 9:33]):
+        with pytest.raises(RuntimeError, match="alias"):
+            ops.grouped_gemm(wide[:, 10:34], w, groups, trans_w=True, out=over)
+    with pytest.raises(RuntimeError, match="alias"):
+        ops.grouped_gemm(x, flat[7000:7000 + 1728].view(3, 24, 24), groups, out=rows)
+    with pytest.raises(RuntimeError, match="alias"):
+        ops.grouped_gemm(x, w, groups, bias=flat[7199:7199 + 72].view(3, 24), out=rows)
+
+
+def test_recorded_backward_beside_an_eager_graph(nn, ops, dev):
+    """A backward pass is recorded after the eager graph of the same layer is gone; while one lives
+    the recording is refused."""
+    layer = nn.GroupedLinear(24, 16, 3).to(dev)
+    x = torch.randn(100, 24, device=dev)
+    groups = ops.group_rows(torch.arange(100, device=dev) % 3, 3)
+    for p in layer.parameters():
+        p.grad = torch.zeros_like(p)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def step():
+        for p in layer.parameters():
+            p.grad.zero_()
+        layer(x, groups).square().sum().backward()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    alive = layer(x, groups).square().sum()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph, stream=side):
+            step()
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for it in range(4):
+        x.copy_(torch.randn(100, 24, device=dev) * (it + 1))
+        graph.replay()
+        got = [p.grad.clone() for p in layer.parameters()]
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, p.grad) for a, p in zip(got, layer.parameters()))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_layer_gradients_match_the_formulas(nn, ops, dev, dtype):
     rows, n_groups, k, n = 777, 5, 40, 24

@@ -42,6 +42,17 @@ def test_host_tensors_are_refused():
     assert float(optim.clip_grad_norm_(p, 1.0)) == 0.0
 
 
+def test_row_groups_are_checked():
+    from torch_geometric_autoscale import ops
+    ptr, order = torch.zeros(3, dtype=torch.int32), torch.arange(4, dtype=torch.int32)
+    assert ops.RowGroups(order, ptr, 4).n_groups == 2
+    for bad in ((order[:3], ptr, 4), (order.long(), ptr, 4), (order, ptr.long(), 4),
+                (order.repeat(2)[::2], ptr, 4), (order, ptr.view(1, 3), 4), (order, ptr[:1], 4),
+                (None, torch.zeros(2050, dtype=torch.int32), 4)):
+        with pytest.raises(ValueError):
+            ops.RowGroups(*bad)
+
+
 def test_layer_parameters():
     from torch_geometric_autoscale import nn
     torch.manual_seed(0)
