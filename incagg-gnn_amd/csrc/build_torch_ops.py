@@ -1,9 +1,9 @@
 #!/usr/bin/env python3
 """Builds the two operator objects the reference package loads by name
 (torch_geometric_autoscale/__init__.py:8-10): ``_relabel.so`` and ``_async.so``, next to this
-package's ``__init__``, and ``_train_ops.so``, this package's own (gradient lists, the grouped linear layer).  All are thin shells over libincagg_gnn.so (csrc/torch_ops.cpp), built
-with the host compiler against the installed torch headers; no GPU is needed to build or load
-them.  Usage: python build_torch_ops.py [--force]"""
+package's ``__init__``, and the module ``_train_ops.so``, this package's own (gradient lists, the
+grouped linear layer).  All are thin shells over libincagg_gnn.so (csrc/torch_ops.cpp), built with
+the host compiler against the installed torch headers; no GPU is needed to build or load them.  Usage: python build_torch_ops.py [--force]"""
 import os
 import subprocess
 import sys
@@ -46,6 +46,8 @@ def build(force: bool = False):
                *inc, SRC, "-o", out, f"-L{torch_lib}", f"-L{LIB_DIR}",
                f"-Wl,-rpath,{torch_lib}", "-Wl,-rpath,$ORIGIN/../lib",
                "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-lincagg_gnn"]
+        if name == "_train_ops":
+            cmd.append("-ltorch_python")
         subprocess.check_call(cmd)
         return out
 

@@ -10,16 +10,21 @@
 // -DINCAGG_OPS_TRAIN builds `_train_ops`, which has no counterpart in the reference: calls whose
 // kernels are shorter than their host side would be in Python -- gradient lists (norm, clipping, the
 // clipped Adam step: a list of ten took longer to walk than the GPU needs for the whole call) and
-// the grouped linear layer with its autograd node.
+// the grouped linear layer with its autograd node.  It is a Python module of plain functions: through
+// the operator registry a call costs 3 us more, and a list 0.2 us a tensor.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 #ifdef INCAGG_OPS_TRAIN
-#include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+
+#include <c10/hip/HIPGraphsC10Utils.h>
 #endif
 
 #include <deque>
@@ -263,7 +268,7 @@ void *current_stream(const at::Device &device) {
   return c10::hip::getCurrentHIPStream(device.index()).stream();
 }
 
-Tensor grad_norm(std::vector<Tensor> grads, int64_t norm_type, double max_norm, bool clip) {
+Tensor grad_norm(const std::vector<Tensor> &grads, int64_t norm_type, double max_norm, bool clip) {
   TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
   const Segments s(grads, clip);
   const at::Device device = grads[0].device();
@@ -282,18 +287,18 @@ Tensor grad_norm(std::vector<Tensor> grads, int64_t norm_type, double max_norm, 
   return scratch.norm;
 }
 
-// hyper: lr, beta1, beta2, eps, weight_decay of every parameter group; group[i]: of tensor i.
-Tensor adam_step_clipped(std::vector<Tensor> params, std::vector<Tensor> grads,
-                         std::vector<Tensor> exp_avg, std::vector<Tensor> exp_avg_sq,
-                         std::vector<Tensor> steps, std::vector<int64_t> group,
-                         std::vector<double> hyper, double max_norm, at::Device device) {
-  const size_t n = params.size();
-  TORCH_CHECK_VALUE(grads.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n &&
-                    steps.size() == n && group.size() == n && hyper.size() % 5 == 0,
-                    "one gradient, two moments, a step count and a group for every parameter");
+// A parameter with its gradient and state; group: its hyperparameters.
+struct AdamTensor {
+  Tensor p, g, m, v, step;
+  int64_t group;
+};
+
+Tensor adam_step_clipped(const std::vector<AdamTensor> &tensors,
+                         const std::vector<incagg_adam_hyper> &hyper, double max_norm,
+                         at::Device device) {
   std::vector<incagg_adam_clip_segment> segs;
   std::vector<Tensor> keep;
-  segs.reserve(n);
+  segs.reserve(tensors.size());
   int64_t elements = 0;
   auto state = [&](const Tensor &t, int64_t numel) {
     TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat && t.device() == device,
@@ -302,26 +307,25 @@ Tensor adam_step_clipped(std::vector<Tensor> params, std::vector<Tensor> grads,
                       "parameters and state must be contiguous and of one size");
     return numel ? static_cast<float *>(t.data_ptr()) : nullptr;
   };
-  for (size_t i = 0; i < n; i++) {
-    Tensor g = grads[i];
-    TORCH_CHECK_TYPE(g.layout() == at::kStrided && g.scalar_type() == at::kFloat &&
-                     g.device() == device, "gradients must be float32 on the parameter's device");
-    const int64_t numel = params[i].numel();
-    TORCH_CHECK_VALUE(g.numel() == numel, "a gradient differs in size from its parameter");
-    if (!g.is_contiguous()) {
-      g = g.detach().contiguous();
-      keep.push_back(g);
+  for (const AdamTensor &t : tensors) {
+    TORCH_CHECK_TYPE(t.g.layout() == at::kStrided && t.g.scalar_type() == at::kFloat &&
+                     t.g.device() == device, "gradients must be float32 on the parameter's device");
+    const int64_t numel = t.p.numel();
+    TORCH_CHECK_VALUE(t.g.numel() == numel, "a gradient differs in size from its parameter");
+    const Tensor *g = &t.g;
+    if (!g->is_contiguous()) {
+      keep.push_back(g->detach().contiguous());
+      g = &keep.back();
     }
-    segs.push_back({state(params[i], numel), numel ? static_cast<const float *>(g.data_ptr()) : nullptr,
-                    state(exp_avg[i], numel), state(exp_avg_sq[i], numel), state(steps[i], 1), numel,
-                    group[i]});
+    segs.push_back({state(t.p, numel), numel ? static_cast<const float *>(g->data_ptr()) : nullptr,
+                    state(t.m, numel), state(t.v, numel), state(t.step, 1), numel, t.group});
     elements += numel;
   }
   c10::DeviceGuard guard(device);
-  Scratch scratch((int64_t)n, elements, device);
+  const int64_t n = (int64_t)segs.size();
+  Scratch scratch(n, elements, device);
   check_status(incagg_adam_step_clipped_f32(
-      segs.data(), (int64_t)n, reinterpret_cast<const incagg_adam_hyper *>(hyper.data()),
-      (int64_t)(hyper.size() / 5), max_norm, scratch.ptr(), scratch.doubles,
+      segs.data(), n, hyper.data(), (int64_t)hyper.size(), max_norm, scratch.ptr(), scratch.doubles,
       scratch.norm.data_ptr<float>(), current_stream(device)));
   return scratch.norm;
 }
@@ -491,21 +495,174 @@ Tensor grouped_linear(const Tensor &x, const Tensor &w, const std::optional<Tens
                     "weight must be [", g, ", out, ", x.size(1), "], got ", w.sizes());
   TORCH_CHECK_VALUE(!bias || (bias->dim() == 2 && bias->size(0) == g && bias->size(1) == w.size(1)),
                     "bias must be [", g, ", ", w.size(1), "]");
+  if (!at::GradMode::is_enabled() ||
+      !(x.requires_grad() || w.requires_grad() || (bias && bias->requires_grad())))
+    return grouped_gemm(x, w, true, bias.value_or(Tensor()), {ptr, order.value_or(Tensor())}, pitch_y);
   return GroupedLinear::apply(x, w, bias, ptr, order, pitch_y, pitch_dx);
 }
+
+// ---- the Python module -------------------------------------------------------------------------
+struct NoGil {
+  PyThreadState *state = PyEval_SaveThread();
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
+
+PyObject *raised(PyObject *o) {
+  if (!o) throw python_error();
+  return o;
+}
+int64_t to_int(PyObject *o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+double to_double(PyObject *o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+const Tensor &to_tensor(PyObject *o, const char *name) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o), name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+std::optional<Tensor> to_optional(PyObject *o, const char *name) {
+  if (o == Py_None) return std::nullopt;
+  return to_tensor(o, name);
+}
+void need_args(Py_ssize_t n, Py_ssize_t want) {
+  TORCH_CHECK_TYPE(n == want, "expected ", want, " arguments, got ", n);
+}
+// An entry of a dict, by a name that is made a string object once.
+PyObject *entry(PyObject *dict, PyObject *key) {
+  TORCH_CHECK_TYPE(PyDict_Check(dict), "parameter groups and states must be dicts");
+  PyObject *v = PyDict_GetItemWithError(dict, key);
+  if (!v && !PyErr_Occurred()) PyErr_SetObject(PyExc_KeyError, key);
+  return raised(v);
+}
+PyObject *name_of(const char *name) { return raised(PyUnicode_InternFromString(name)); }
+
+// (parameters: list, norm_type, max_norm, clip) -> norm, None without a gradient
+PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 4);
+  TORCH_CHECK_TYPE(PyList_Check(args[0]), "parameters must be a list");
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  std::vector<Tensor> grads;
+  grads.reserve(n);
+  for (Py_ssize_t i = 0; i < n; i++) {
+    const Tensor &g = to_tensor(PyList_GET_ITEM(args[0], i), "a parameter").grad();
+    if (g.defined()) grads.push_back(g);
+  }
+  if (grads.empty()) Py_RETURN_NONE;
+  const int64_t norm_type = to_int(args[1]);
+  const double max_norm = to_double(args[2]);
+  const bool clip = args[3] == Py_True;
+  Tensor norm;
+  {
+    NoGil unlocked;
+    norm = grad_norm(grads, norm_type, max_norm, clip);
+  }
+  return THPVariable_Wrap(norm);
+  END_HANDLE_TH_ERRORS
+}
+
+// (param_groups: list of dicts, states: per group a list of the parameters' state dicts, max_norm)
+PyObject *py_adam_step_clipped(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  static PyObject *const k_params = name_of("params"), *const k_lr = name_of("lr"),
+                  *const k_betas = name_of("betas"), *const k_eps = name_of("eps"),
+                  *const k_decay = name_of("weight_decay"), *const k_m = name_of("exp_avg"),
+                  *const k_v = name_of("exp_avg_sq"), *const k_step = name_of("step");
+  need_args(n_args, 3);
+  TORCH_CHECK_TYPE(PyList_Check(args[0]) && PyList_Check(args[1]) &&
+                   PyList_GET_SIZE(args[0]) == PyList_GET_SIZE(args[1]),
+                   "one list of states for every parameter group");
+  std::vector<incagg_adam_hyper> hyper;
+  std::vector<AdamTensor> tensors;
+  std::optional<at::Device> device;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); i++) {
+    PyObject *group = PyList_GET_ITEM(args[0], i), *states = PyList_GET_ITEM(args[1], i);
+    PyObject *params = entry(group, k_params), *betas = entry(group, k_betas);
+    TORCH_CHECK_TYPE(PyList_Check(params) && PyList_Check(states), "params must be a list");
+    TORCH_CHECK_VALUE(PyList_GET_SIZE(params) == PyList_GET_SIZE(states),
+                      "a group's parameters have changed since the optimizer was made");
+    TORCH_CHECK_TYPE(PySequence_Check(betas) && PySequence_Size(betas) == 2, "betas must be a pair");
+    THPObjectPtr b1(raised(PySequence_GetItem(betas, 0))), b2(raised(PySequence_GetItem(betas, 1)));
+    hyper.push_back({to_double(entry(group, k_lr)), to_double(b1.get()), to_double(b2.get()),
+                     to_double(entry(group, k_eps)), to_double(entry(group, k_decay))});
+    for (Py_ssize_t j = 0; j < PyList_GET_SIZE(params); j++) {
+      const Tensor &p = to_tensor(PyList_GET_ITEM(params, j), "a parameter"), &g = p.grad();
+      if (!device) device = p.device();
+      if (!g.defined()) continue;
+      PyObject *state = PyList_GET_ITEM(states, j);
+      tensors.push_back({p, g, to_tensor(entry(state, k_m), "exp_avg"),
+                         to_tensor(entry(state, k_v), "exp_avg_sq"),
+                         to_tensor(entry(state, k_step), "step"), (int64_t)i});
+    }
+  }
+  TORCH_CHECK_VALUE(device, "no parameters");
+  const double max_norm = to_double(args[2]);
+  Tensor norm;
+  {
+    NoGil unlocked;
+    norm = adam_step_clipped(tensors, hyper, max_norm, *device);
+  }
+  return THPVariable_Wrap(norm);
+  END_HANDLE_TH_ERRORS
+}
+
+// (ids, n_groups) -> order, ptr
+PyObject *py_group_rows(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 2);
+  const Tensor ids = to_tensor(args[0], "ids");
+  const int64_t n_groups = to_int(args[1]);
+  std::tuple<Tensor, Tensor> r;
+  {
+    NoGil unlocked;
+    r = group_rows(ids, n_groups);
+  }
+  THPObjectPtr order(raised(THPVariable_Wrap(std::get<0>(r))));
+  THPObjectPtr ptr(raised(THPVariable_Wrap(std::get<1>(r))));
+  return PyTuple_Pack(2, order.get(), ptr.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, weight, bias or None, ptr, order or None, n_rows, pitch_y, pitch_dx) -> y
+PyObject *py_grouped_linear(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  need_args(n_args, 8);
+  const Tensor x = to_tensor(args[0], "x"), w = to_tensor(args[1], "weight");
+  const std::optional<Tensor> bias = to_optional(args[2], "bias");
+  const Tensor ptr = to_tensor(args[3], "ptr");
+  const std::optional<Tensor> order = to_optional(args[4], "order");
+  const int64_t n_rows = to_int(args[5]), pitch_y = to_int(args[6]), pitch_dx = to_int(args[7]);
+  Tensor y;
+  {
+    NoGil unlocked;
+    y = grouped_linear(x, w, bias, ptr, order, n_rows, pitch_y, pitch_dx);
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+template <typename F> PyCFunction function(F f) {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
+}
+PyMethodDef g_functions[] = {
+    {"grad_norm", function(py_grad_norm), METH_FASTCALL, nullptr},
+    {"adam_step_clipped", function(py_adam_step_clipped), METH_FASTCALL, nullptr},
+    {"group_rows", function(py_group_rows), METH_FASTCALL, nullptr},
+    {"grouped_linear", function(py_grouped_linear), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_train_ops", nullptr, -1, g_functions};
 #endif  // INCAGG_OPS_TRAIN
 
 }  // namespace
 
 #ifdef INCAGG_OPS_TRAIN
-TORCH_LIBRARY(incagg_train, m) {
-  m.def("grad_norm(Tensor[] grads, int norm_type, float max_norm, bool clip) -> Tensor", &grad_norm);
-  m.def("adam_step_clipped(Tensor[] params, Tensor[] grads, Tensor[] exp_avg, Tensor[] exp_avg_sq, "
-        "Tensor[] steps, int[] group, float[] hyper, float max_norm, Device device) -> Tensor",
-        &adam_step_clipped);
-  m.def("group_rows(Tensor ids, int n_groups) -> (Tensor, Tensor)", &group_rows);
-  m.def("grouped_linear(Tensor x, Tensor weight, Tensor? bias, Tensor ptr, Tensor? order, int n_rows, "
-        "int pitch_y, int pitch_dx) -> Tensor", &grouped_linear);
+extern "C" __attribute__((visibility("default"))) PyObject *PyInit__train_ops() {
+  return PyModule_Create(&g_module);
 }
 #else
 // Both objects contribute to one namespace, hence fragments.

@@ -8,6 +8,7 @@ reference's native extension are registered under the same names in
 """
 import collections
 import ctypes
+import importlib
 import os
 from typing import Optional, Tuple
 
@@ -734,14 +735,12 @@ def softmax_cross_entropy(logits: Tensor, labels: Tensor) -> Tensor:
 
 
 # --------------------------------------------------------------------------- rows of several kinds
-TrainOps = collections.namedtuple("TrainOps",
-                                  "grad_norm adam_step_clipped group_rows grouped_linear")
 _train_ops = None
 
 
-def train_ops() -> TrainOps:
-    """The operator object `_train_ops.so` (csrc/build_torch_ops.py): calls over the C ABI whose
-    host side in Python would take longer than their kernels."""
+def train_ops():
+    """The module `_train_ops.so` (csrc/build_torch_ops.py): calls over the C ABI whose host side in
+    Python would take longer than their kernels."""
     global _train_ops
     if _train_ops is None:
         path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_train_ops.so")
@@ -749,9 +748,7 @@ def train_ops() -> TrainOps:
             raise _lib.IncAggLibraryError(
                 f"{path} not found: build it with `python incagg-gnn_amd/csrc/build_torch_ops.py` "
                 "(there is no fallback implementation)")
-        torch.ops.load_library(path)
-        ns = torch.ops.incagg_train
-        _train_ops = TrainOps(*(getattr(ns, name).default for name in TrainOps._fields))
+        _train_ops = importlib.import_module("._train_ops", __package__)
     return _train_ops
 
 

@@ -34,10 +34,8 @@ def _max_norm(max_norm) -> float:
     return max_norm
 
 
-def _gradients(parameters) -> List[Tensor]:
-    if isinstance(parameters, Tensor):
-        parameters = (parameters,)
-    return [g for g in [p.grad for p in parameters] if g is not None]
+def _list(parameters) -> List[Tensor]:
+    return [parameters] if isinstance(parameters, Tensor) else list(parameters)
 
 
 def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0) -> Tensor:
@@ -46,8 +44,8 @@ def grad_norm(parameters: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.
     fixed order.  float32, bfloat16 and float16 gradients may be mixed.  ``norm_type``: 2, 1 or
     ``inf``."""
     code = _norm_type(norm_type)
-    grads = _gradients(parameters)
-    return ops.train_ops().grad_norm(grads, code, 0.0, False) if grads else torch.zeros(())
+    norm = ops.train_ops().grad_norm(_list(parameters), code, 0.0, False)
+    return torch.zeros(()) if norm is None else norm
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
@@ -58,14 +56,14 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     overlap in memory.  ``error_if_nonfinite`` waits for the GPU, and raises before anything is
     scaled.  An optimizer step right behind it can clip as it reads: :meth:`Adam.step`."""
     code, max_norm = _norm_type(norm_type), _max_norm(max_norm)
-    grads = _gradients(parameters)
-    if not grads:
-        return torch.zeros(())
-    call = ops.train_ops().grad_norm
-    if error_if_nonfinite and not bool(torch.isfinite(call(grads, code, 0.0, False))):
-        raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is "
-                           "non-finite, so it cannot be clipped")
-    return call(grads, code, max_norm, True)
+    parameters, call = _list(parameters), ops.train_ops().grad_norm
+    if error_if_nonfinite:
+        norm = call(parameters, code, 0.0, False)
+        if norm is not None and not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is "
+                               "non-finite, so it cannot be clipped")
+    norm = call(parameters, code, max_norm, True)
+    return torch.zeros(()) if norm is None else norm
 
 
 class Adam:
@@ -132,7 +130,8 @@ class Adam:
         are read -- ``clip_grad_norm_`` and the step in two launches; ``p.grad`` itself stays as
         it is -- and the norm they had is returned (a scalar on the device)."""
         if max_norm is not None:
-            return self._clipped_step(_max_norm(max_norm))
+            return ops.train_ops().adam_step_clipped(self.param_groups, self._states,
+                                                     _max_norm(max_norm))
         return self._plain_step()
 
     @torch.no_grad()
@@ -160,22 +159,6 @@ class Adam:
                 _lib.check(L.incagg_adam_step_f32(
                     ctypes.addressof(segs), len(with_grad), group["lr"], b1, b2, group["eps"],
                     group["weight_decay"], ops._stream_of(self.device)))
-
-    def _clipped_step(self, max_norm: float) -> Tensor:
-        params, states, group_of, hyper = [], [], [], []
-        for i, group in enumerate(self.param_groups):
-            hyper += (group["lr"], *group["betas"], group["eps"], group["weight_decay"])
-            params += group["params"]
-            states += self._states[i]
-            group_of += [i] * len(group["params"])
-        grads = [p.grad for p in params]
-        if any(g is None for g in grads):
-            live = [k for k, g in enumerate(grads) if g is not None]
-            params, states, group_of, grads = ([v[k] for k in live]
-                                               for v in (params, states, group_of, grads))
-        return ops.train_ops().adam_step_clipped(params, grads, [st["exp_avg"] for st in states],
-                              [st["exp_avg_sq"] for st in states], [st["step"] for st in states],
-                              group_of, hyper, max_norm, self.device)
 
     def state_dict(self) -> dict:
         return {"param_groups": [{k: (v.clone() if isinstance(v, Tensor) else v)
