@@ -112,21 +112,17 @@ __device__ inline void put_split(unsigned short *tile, int at, const float (&v)[
   *reinterpret_cast<u4 *>(tile + 2 * PLANE + at) = l;
 }
 
-// 16 bytes shifted down by `bits` (0 .. 128), zeros behind.
-__device__ inline Pack<unsigned, 4> shift_down(Pack<unsigned, 4> v, int bits) {
-  typedef unsigned long long u64;
-  u64 lo = v.v[0] | (u64)v.v[1] << 32, hi = v.v[2] | (u64)v.v[3] << 32;
-  if (bits >= 64) {
-    lo = hi;
-    hi = 0;
-    bits -= 64;
+// 16 bytes shifted down by `halves` times 16 bits (0 .. 8), zeros behind.
+__device__ inline void shift_down(unsigned *v, int halves) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = halves & 2 ? (e < 3 ? v[e + 1] : 0u) : v[e];
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = halves & 4 ? (e < 2 ? v[e + 2] : 0u) : v[e];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const unsigned odd = v[e] >> 16 | (e < 3 ? v[e + 1] << 16 : 0u);
+    v[e] = halves & 8 ? 0u : (halves & 1 ? odd : v[e]);
   }
-  if (bits >= 64) lo = 0;
-  else if (bits > 0) {
-    lo = lo >> bits | hi << (64 - bits);
-    hi >>= bits;
-  }
-  return {{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)}};
 }
 
 // Loads at ragged edges are whole vectors as well, of what lies in front of the edge, shifted: a
@@ -153,31 +149,42 @@ template <int D, int ROWS, int THREADS> struct RowStage {
       r[i] = __builtin_bit_cast(Pack<unsigned, W>,
                                 *reinterpret_cast<const Pack<Raw, 8> *>(src[i] + k0));
   }
-  // the last chunk of a row of k values
+  // the last chunk of a row of k values; settle() moves them to where they belong
+  static constexpr int N = 16 / sizeof(Raw);    // values of a load
   __device__ void load_tail(int k0, int k) {
-    constexpr int N = 16 / sizeof(Raw);
 #pragma unroll
     for (int i = 0; i < U; i++) {
       const int at = (unit(i) % CH) * 8;
       const Raw *row = src[i] - at;
 #pragma unroll
       for (int h = 0; h < 8; h += N) {
-        const int left = k - k0 - at - h;           // values from here to the row's end
         Pack<unsigned, 4> q;
         if (k >= N) {
           q = *reinterpret_cast<const Pack<unsigned, 4> *>(
-              reinterpret_cast<const Pack<Raw, N> *>(row + (left >= N ? k0 + at + h : k - N)));
-          q = shift_down(q, (N - min(max(left, 0), N)) * 8 * (int)sizeof(Raw));
+              reinterpret_cast<const Pack<Raw, N> *>(row + min(k0 + at + h, k - N)));
         } else {
           Pack<Raw, N> v;
 #pragma unroll
-          for (int e = 0; e < N; e++) v.v[e] = e < left ? row[k0 + at + h + e] : (Raw)0;
+          for (int e = 0; e < N; e++) v.v[e] = at + h + e < k ? row[at + h + e] : (Raw)0;
           q = __builtin_bit_cast(Pack<unsigned, 4>, v);
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) r[i].v[h * (int)sizeof(Raw) / 4 + e] = q.v[e];
       }
     }
+  }
+  // in front of the store of a chunk with `left` values along k: where the values are waited for
+  // anyhow (at the load, the wait would stand in front of the products of the chunk before)
+  __device__ void settle(int left, int k) {
+    if (left >= BK || k < N) return;
+#pragma unroll
+    for (int i = 0; i < U; i++)
+#pragma unroll
+      for (int h = 0; h < 8; h += N) {
+        const int here = left - (unit(i) % CH) * 8 - h;       // values from here to the row's end
+        shift_down(&r[i].v[h * (int)sizeof(Raw) / 4],
+                   (N - min(max(here, 0), N)) * ((int)sizeof(Raw) / 2));
+      }
   }
   __device__ void store(unsigned short *tile) {
 #pragma unroll
@@ -203,19 +210,17 @@ template <int D, int COLS, int THREADS> struct ColStage {
   static_assert(V >= 1 && V <= 4 && GROUPS * (BK / 8) == THREADS, "every thread takes 8 x V values");
   typedef Raw Row __attribute__((ext_vector_type(V)));
   Row r[8];
-  int at, shift, cols;                  // where this thread's columns are loaded from, moved by what
-  bool narrow;                          // a matrix of fewer columns than a vector has
+  int at, shift;                        // where this thread's columns are loaded from, moved by what
   static __device__ int col() { return ((int)threadIdx.x % GROUPS) * V; }
   static __device__ int row() { return ((int)threadIdx.x / GROUPS) * 8; }
   __device__ void init(int first, int n) {
-    narrow = n < V;
-    cols = n - first - col();
-    at = narrow ? first + col() : min(first + col(), n - V);
-    shift = narrow || cols <= 0 ? 0 : first + col() - at;   // (columns behind the last: dropped)
+    const int begin = first + col();
+    at = n < V ? begin : min(begin, n - V);
+    shift = begin >= n ? 0 : begin - at;        // (columns behind the last: dropped)
   }
-  // row i (0 .. 7) of this thread starts at row_of(i), which has to be a row of the matrix
-  template <typename F> __device__ void load(F &&row_of) {
-    if (!narrow) {
+  // row i (0 .. 7) of this thread starts at row_of(i), which has to be a row of the matrix of n columns
+  template <typename F> __device__ void load(int n, F &&row_of) {
+    if (n >= V) {
 #pragma unroll
       for (int i = 0; i < 8; i++)
         r[i] = __builtin_bit_cast(Row, *reinterpret_cast<const Pack<Raw, V> *>(row_of(i) + at));
@@ -224,7 +229,7 @@ template <int D, int COLS, int THREADS> struct ColStage {
       for (int i = 0; i < 8; i++) {
         const Raw *p = row_of(i) + at;
 #pragma unroll
-        for (int e = 0; e < V; e++) r[i][e] = e < cols ? p[e] : (Raw)0;
+        for (int e = 0; e < V; e++) r[i][e] = at + e < n ? p[e] : (Raw)0;
       }
     }
   }
@@ -550,9 +555,9 @@ void grouped_rows_kernel(const GroupedArgs a) {
         const int r0 = k0 + wc[f].row();
         if (k0 + BK <= a.k) {
           const Raw *p = w + (long long)r0 * a.ldw;
-          wc[f].load([&](int i) { return p + i * a.ldw; });
+          wc[f].load(a.n, [&](int i) { return p + i * a.ldw; });
         } else {
-          wc[f].load([&](int i) { return w + (long long)min(r0 + i, a.k - 1) * a.ldw; });
+          wc[f].load(a.n, [&](int i) { return w + (long long)min(r0 + i, a.k - 1) * a.ldw; });
           wc[f].clear_from(a.k - r0);
         }
       }
@@ -565,9 +570,11 @@ void grouped_rows_kernel(const GroupedArgs a) {
       load_x(c, f);
       load_w(c, f);
     };
-    auto store = [&](int s, int f) __attribute__((always_inline)) {
+    auto store = [&](int c, int s, int f) __attribute__((always_inline)) {
+      xs[f].settle(a.k - c * BK, a.k);
       xs[f].store(xt + s * P * BM * BK);
       if constexpr (TRANS_W) {
+        wr[f].settle(a.k - c * BK, a.k);
         wr[f].store(wt + s * P * BN * BK);
       } else {
         wc[f].settle();
@@ -591,7 +598,7 @@ void grouped_rows_kernel(const GroupedArgs a) {
           const int c = c0 + u;
           if (c >= n_chunks) break;
           // (the other buffer may still be read; this one was read before the last barrier)
-          store(u & 1, u % FLIGHT);
+          store(c, u & 1, u % FLIGHT);
           __syncthreads();
           if (c + FLIGHT < n_chunks) load(c + FLIGHT, u % FLIGHT);
           multiply<D, BM, BN>(xt + (u & 1) * P * BM * BK, wt + (u & 1) * P * BN * BK, row0, col0, acc);
@@ -600,7 +607,7 @@ void grouped_rows_kernel(const GroupedArgs a) {
       static_assert(FLIGHT == 1, "one buffer, one chunk on its way");
       for (int c = 0; c < n_chunks; c++) {
         if (c > 0) __syncthreads();
-        store(0, 0);
+        store(c, 0, 0);
         __syncthreads();
         if (c + 1 < n_chunks) load(c + 1, 0);
         multiply<D, BM, BN>(xt, wt, row0, col0, acc);
@@ -717,6 +724,7 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
   const int *const order = t.order;
   const long long lda = t.lda, ldb = t.ldb;
   const unsigned last_row = t.rows - 1u;
+  const int width_a = t.m, width_b = t.n;
   as.init(m0, t.m);
   bs.init(n0, t.n);
   // row numbers of a chunk are fetched one chunk ahead of its rows
@@ -739,13 +747,13 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
     const int ra = r0 + as.row(), rb = r0 + bs.row();
     // (rows behind the last repeat it, row numbers outside the matrix its last row: cleared below)
     if (order) {
-      as.load([&](int i) { return a + (long long)min((unsigned)ia[i], last_row) * lda; });
-      bs.load([&](int i) { return b + (long long)min((unsigned)ib[i], last_row) * ldb; });
+      as.load(width_a, [&](int i) { return a + (long long)min((unsigned)ia[i], last_row) * lda; });
+      bs.load(width_b, [&](int i) { return b + (long long)min((unsigned)ib[i], last_row) * ldb; });
     } else {
       const int la = last - 1 - ra, lb = last - 1 - rb;
       const Raw *pa = a + (long long)min(ra, last - 1) * lda, *pb = b + (long long)min(rb, last - 1) * ldb;
-      as.load([&](int i) { return i <= la ? pa + i * lda : pa; });
-      bs.load([&](int i) { return i <= lb ? pb + i * ldb : pb; });
+      as.load(width_a, [&](int i) { return i <= la ? pa + i * lda : pa; });
+      bs.load(width_b, [&](int i) { return i <= lb ? pb + i * ldb : pb; });
     }
     if (r0 + BK > last) {
       as.clear_from(last - ra);
