@@ -1288,13 +1288,24 @@ static bool tn_large_tiles(int64_t m, int64_t n, int dtype) {
 
 // Rows of a segment: enough segments to fill the chip (one workgroup to a CU of 256 x 256 tiles,
 // two of 128 x 128), at least 256 rows.  Shorter ones even out groups of different sizes, but every
-// one of a longer group costs a partial written and read.
-static int tn_segment(int64_t rows, int64_t m, int64_t n, int dtype) {
+// one of a longer group costs a partial written and read (float32, 16326 rows, 256 x 256, 128 / 256 /
+// 512 rows: 46 / 41 / 49 us).  A group ends inside a segment, which makes up to one more for each.
+// Where a group has many segments (`even`) those would be the few workgroups over a full round that
+// cost another one: there they are taken off (without / with, 60000 rows in 5 groups, 512 x 512
+// bfloat16 113 / 73 us; 65304 rows in 5 groups, 256 x 256 float32 132 / 93).  Where it has few, short
+// last segments make room early (20000 rows in 8 groups, 1024 x 1024 float16 144 / 164).
+struct Segments {
+  int rows;
+  bool even;
+};
+static Segments tn_segments(int64_t rows, int64_t n_groups, int64_t m, int64_t n, int dtype) {
   const bool large = tn_large_tiles(m, n, dtype);
   const int64_t tile = large ? 256 : 128, tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
   const int64_t wanted = std::max<int64_t>(1, (large ? 256 : 512) / tiles);
-  const int64_t s = std::max<int64_t>(256, (rows + wanted - 1) / wanted);
-  return (int)((s + 63) / 64 * 64);
+  const bool even = n_groups * 8 <= wanted && rows >= 256 * wanted;
+  const int64_t count = even ? wanted - n_groups : wanted;
+  const int64_t s = std::max<int64_t>(256, (rows + count - 1) / count);
+  return {(int)((s + 63) / 64 * 64), even};
 }
 
 // Adds up the partials of groups that were cut into segments.
@@ -1330,20 +1341,21 @@ static int launch_tn_lds(TnArgs &t, hipStream_t s) {
   return tn_finish<D>(t, s);
 }
 
-template <int D> static int launch_tn(TnArgs &t, hipStream_t s) {
+template <int D> static int launch_tn(TnArgs &t, bool even, hipStream_t s) {
   if constexpr (D != INCAGG_DTYPE_F32) {
     if (tn_large_tiles(t.m, t.n, D) && pieces(t.a, t.lda, t.m) && pieces(t.b, t.ldb, t.n))
       return launch_tn_lds<D, 256, 256, 2, 4>(t, s);
   }
   if (t.n <= 64) return t.m <= 64 ? launch_tn_tile<D, 64, 64>(t, s) : launch_tn_tile<D, 128, 64>(t, s);
   // 128 x 128 tiles load and split less for a product, 64 x 128 leave twice the workgroups to hide
-  // what they wait for.  float32, us by 128 / 64: 16326 rows, 256 x 256 46 / 42, 65304 rows 121 / 112;
-  // 65536 rows, 1024 x 1024 1036 / 1236, 40000 rows in 40 groups, 512 x 512 228 / 244; one column of
-  // tiles, 128064 rows, 256 x 100, 82 / 94.  float16 30000 rows, 300 x 601 174 / 125; bfloat16 30000
-  // rows, 256 x 100 38 / 23.
+  // what they wait for.  float32, us by 128 / 64: 16326 rows, 256 x 256 46 / 41, even segments: 65304
+  // rows, 256 x 256 93 / 110, 100000 rows, 300 x 200 154 / 188; 65536 rows, 1024 x 1024 1114 / 1195, 40000
+  // rows in 40 groups, 512 x 512 226 / 210; one column of tiles, 128064 rows, 256 x 100, 83 / 100.
+  // 16-bit types always take the narrower: float16 30000 rows, 300 x 601 250 / 74; bfloat16 30000
+  // rows, 256 x 100 57 / 23.
   if constexpr (D == INCAGG_DTYPE_F32) {
     const int64_t tiles = (int64_t)((t.m + 127) / 128) * ((t.n + 127) / 128);
-    if (t.m > 64 && (t.n <= 128 || (t.rows / t.segment + t.n_groups) * tiles >= 800))
+    if (t.m > 64 && (t.n <= 128 || even || (t.rows / t.segment + t.n_groups) * tiles >= 800))
       return launch_tn_tile<D, 128, 128>(t, s);
   }
   return launch_tn_tile<D, 64, 128>(t, s);
@@ -1396,7 +1408,7 @@ extern "C" int64_t incagg_grouped_tn_ws_bytes(int64_t n_groups, int64_t rows, in
   if (n_groups < 1 || rows < 0 || rows > INT_MAX - 4096 || m < 1 || n < 1 || m >= (1 << 20) ||
       n >= (1 << 20))
     return fail(INCAGG_E_INVALID, "size out of range");
-  const int64_t segment = tn_segment(rows, m, n, dtype);
+  const int64_t segment = tn_segments(rows, n_groups, m, n, dtype).rows;
   return rows <= segment ? 0 : (3 * rows / segment + 1) * (m * n + m) * (int64_t)sizeof(float);
 }
 
@@ -1418,7 +1430,8 @@ extern "C" int incagg_grouped_tn(const void *a, int64_t lda, const void *b, int6
                  (long long)ws_bytes, (long long)need);
   TnArgs t{};
   t.partials = static_cast<float *>(ws);
-  t.segment = tn_segment(rows, m, n, dtype);
+  const Segments segments = tn_segments(rows, n_groups, m, n, dtype);
+  t.segment = segments.rows;
   t.a = a; t.b = b; t.d = d; t.sums = sums; t.lda = lda; t.ldb = ldb; t.d_group = d_group;
   t.ptr = ptr; t.order = order; t.n_groups = (int)n_groups; t.rows = (int)rows;
   t.m = (int)m; t.n = (int)n;
@@ -1426,8 +1439,8 @@ extern "C" int incagg_grouped_tn(const void *a, int64_t lda, const void *b, int6
   if (rc) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case INCAGG_DTYPE_F32: return launch_tn<INCAGG_DTYPE_F32>(t, s);
-    case INCAGG_DTYPE_BF16: return launch_tn<INCAGG_DTYPE_BF16>(t, s);
-    default: return launch_tn<INCAGG_DTYPE_F16>(t, s);
+    case INCAGG_DTYPE_F32: return launch_tn<INCAGG_DTYPE_F32>(t, segments.even, s);
+    case INCAGG_DTYPE_BF16: return launch_tn<INCAGG_DTYPE_BF16>(t, segments.even, s);
+    default: return launch_tn<INCAGG_DTYPE_F16>(t, segments.even, s);
   }
 }
