@@ -495,8 +495,11 @@ Tensor grouped_linear(const Tensor &x, const Tensor &w, const std::optional<Tens
                     "weight must be [", g, ", out, ", x.size(1), "], got ", w.sizes());
   TORCH_CHECK_VALUE(!bias || (bias->dim() == 2 && bias->size(0) == g && bias->size(1) == w.size(1)),
                     "bias must be [", g, ", ", w.size(1), "]");
-  if (!at::GradMode::is_enabled() ||
-      !(x.requires_grad() || w.requires_grad() || (bias && bias->requires_grad())))
+  const bool recorded = x.requires_grad() || w.requires_grad() || (bias && bias->requires_grad());
+  // (forward-mode derivatives are refused by the node, which has none)
+  const bool dual = x._fw_grad(0).defined() || w._fw_grad(0).defined() ||
+                    (bias && bias->_fw_grad(0).defined());
+  if (!dual && !(recorded && at::GradMode::is_enabled()))
     return grouped_gemm(x, w, true, bias.value_or(Tensor()), {ptr, order.value_or(Tensor())}, pitch_y);
   return GroupedLinear::apply(x, w, bias, ptr, order, pitch_y, pitch_dx);
 }

@@ -528,6 +528,19 @@ def test_second_derivatives_are_refused(nn, ops, dev):
         g.sum().backward()
 
 
+def test_forward_mode_derivatives_are_refused(nn, ops, dev):
+    from torch.autograd import forward_ad
+    layer = nn.GroupedLinear(8, 4, 2).to(dev).requires_grad_(False)
+    groups = ops.group_rows(torch.arange(10, device=dev) % 2, 2)
+    x = torch.randn(10, 8, device=dev)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, NotImplementedError)):
+                layer(dual, groups)
+    assert layer(x, groups).shape == (10, 4)
+
+
 def test_recorded_products_replay(nn, ops, dev):
     """Ordering, forward and gradients recorded into a HIP graph: replays see new rows AND new
     groups, with eager calls of the same operators in between."""
