@@ -50,7 +50,7 @@ struct TnArgs {
   float *partials;
   long long lda, ldb, d_group;
   const int *ptr, *order;
-  int n_groups, rows, m, n, m_tiles, n_tiles, segment;
+  int n_groups, rows, m, n, m_tiles, n_tiles, segment, slots;
   int *err;
 };
 
@@ -446,6 +446,13 @@ __device__ inline bool tile_of_slot(const int *ptr, int n_groups, int rows, int 
 __device__ inline int xcd_contiguous(int block, int blocks) {
   const int xcd = block & 7, per = blocks >> 3, rem = blocks & 7;
   return xcd * per + min(xcd, rem) + (block >> 3);
+}
+
+// The same where the work comes in units of unequal length, `tiles` workgroups each: unit u goes to
+// XCD u % 8, so that no XCD gets the long ones.  -1: behind the last unit.
+__device__ inline int xcd_spread(int block, int units, int tiles) {
+  const int at = block >> 3, unit = (at / tiles) * 8 + (block & 7);
+  return unit < units ? unit * tiles + at % tiles : -1;
 }
 
 // A row number of `order`, -1 (and reported) outside the matrix.
@@ -1069,7 +1076,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_tn_lds_kernel(const T
   static_assert(A::PER * A::ROWS == B::PER * B::ROWS, "a wave loads the same rows of both");
   constexpr int WAVE_ROWS = A::PER * A::ROWS;
   __shared__ __align__(1024) unsigned short tiles[2 * Pipe::CHUNK];
-  const int work = xcd_contiguous(blockIdx.x, gridDim.x);
+  // (segments of different length: 131072 rows in 16 groups, 1024 x 2048, contiguous / spread 823 / 725 us,
+  // 65536 rows in one, 2048 x 2048 1107 / 640; a unit is a row of tiles, which share their part of A)
+  const int work = xcd_spread(blockIdx.x, t.slots * t.m_tiles, t.n_tiles);
+  if (work < 0) return;
   const int per_slot = t.m_tiles * t.n_tiles, slot = work / per_slot, mn = work - slot * per_slot;
   const int m0 = (mn / t.n_tiles) * BM, n0 = (mn % t.n_tiles) * BN;
   int g, first, end, seg;
@@ -1333,7 +1343,8 @@ template <int D, int BM, int BN, int WM, int WN>
 static int launch_tn_lds(TnArgs &t, hipStream_t s) {
   t.m_tiles = (t.m + BM - 1) / BM;
   t.n_tiles = (t.n + BN - 1) / BN;
-  const int64_t blocks = ((int64_t)t.rows / t.segment + t.n_groups) * t.m_tiles * t.n_tiles;
+  t.slots = t.rows / t.segment + t.n_groups;
+  const int64_t blocks = ((int64_t)t.slots * t.m_tiles + 7) / 8 * 8 * t.n_tiles;
   INCAGG_REQUIRE(blocks * (64 * WM * WN) < kMaxThreads, "too many rows and columns for one call");
   hipLaunchKernelGGL((grouped_tn_lds_kernel<D, BM, BN, WM, WN>), dim3((unsigned)blocks),
                      dim3(64 * WM * WN), 0, s, t);
