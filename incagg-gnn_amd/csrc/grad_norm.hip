@@ -5,12 +5,12 @@
 //     coef  = min(1, max_norm / (total + 1e-6))
 //     clip:  x_t[i] *= coef            Adam:  g' = coef g + wd p, then torch.optim.Adam's update
 //
-// Two launches each (more for more than 128 tensors, 64 in Adam's second).  The first sums: every workgroup walks units of 8192 consecutive elements of
-// ONE tensor and leaves one partial in the caller's workspace.  The second clips (or updates), and
-// every one of its workgroups first adds up all partials by itself, in a fixed order: at most 1024
-// doubles from the L2 for 128 tensors, a microsecond, where a finishing launch would cost several and a
-// last-arriver counter would be state that two recorded graphs share.  Same order everywhere and
-// every time: the same bits.
+// Two launches each (more for more than 128 tensors, 64 in Adam's second).  The first sums: every
+// workgroup walks units of 8192 consecutive elements of ONE tensor and leaves one partial in the
+// caller's workspace.  The second clips (or updates), and every one of its workgroups first adds up
+// all partials by itself, in a fixed order: at most 1024 doubles from the L2 for 128 tensors, a
+// microsecond, where a finishing launch would cost several and a last-arriver counter would be state
+// that two recorded graphs share.  Same order everywhere and every time: the same bits.
 //
 // Numerics: sums and the total are held in 64 bits, so neither the square of a large float32
 // value nor the sum of 10^9 small ones loses anything (the float64 pipes keep up: a multiply-add
@@ -19,8 +19,8 @@
 //
 // Bound by memory once there is enough of it.  200 M elements in 300 tensors of three types: norm 107
 // us (read at 5.6 TB/s), norm and scaling 258 us; Adam with clipping over 64 M parameters 412 us (28
-// bytes each at 5.1 TB/s: 351 us, and the norm in front of it).  Small ones are two launches: 10 tensors of
-// 110 k elements 12.5 us, Adam over 20 tensors of 1.1 M 15.6 us, most of both on the host.
+// bytes each at 5.1 TB/s: 351 us, and the norm in front of it).  Small ones are two launches: 10
+// tensors of 110 k elements 12.5 us, Adam over 20 tensors of 1.1 M 15.6 us, most of both on the host.
 #include "common.h"
 
 #include <hip/hip_bf16.h>
