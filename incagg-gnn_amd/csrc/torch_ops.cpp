@@ -569,7 +569,37 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// (param_groups: list of dicts, states: per group a list of the parameters' state dicts, max_norm)
+// Looks up the parameters' states in the optimizer's own mapping, every time: it belongs to the user,
+// who may replace a state or reorder the parameters between two steps.  The entries usually stand in
+// the order in which the parameters are asked for, so the next one is tried first: finding a tensor by
+// its hash is a call into Python, a fifth of a small step for twenty of them.
+class StateWalk {
+  PyObject *states_;
+  Py_ssize_t next_ = 0;
+
+  // The next entry's state if the entry is this parameter's, which is passed then.
+  PyObject *pass(PyObject *parameter) {
+    if (!PyDict_CheckExact(states_)) return nullptr;
+    Py_ssize_t at = next_;
+    PyObject *key, *value;
+    if (!PyDict_Next(states_, &at, &key, &value) || key != parameter) return nullptr;
+    next_ = at;
+    return value;
+  }
+
+ public:
+  explicit StateWalk(PyObject *states) : states_(states) {}
+  void skip(PyObject *parameter) { pass(parameter); }
+  PyObject *of(PyObject *parameter) {             // (a new reference)
+    if (PyObject *state = pass(parameter)) {
+      Py_INCREF(state);
+      return state;
+    }
+    return raised(PyObject_GetItem(states_, parameter));      // KeyError where there is none
+  }
+};
+
+// (param_groups: list of dicts, state: mapping of the parameters to their state dicts, max_norm)
 PyObject *py_adam_step_clipped(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   static PyObject *const k_params = name_of("params"), *const k_lr = name_of("lr"),
@@ -577,27 +607,28 @@ PyObject *py_adam_step_clipped(PyObject *, PyObject *const *args, Py_ssize_t n_a
                   *const k_decay = name_of("weight_decay"), *const k_m = name_of("exp_avg"),
                   *const k_v = name_of("exp_avg_sq"), *const k_step = name_of("step");
   need_args(n_args, 3);
-  TORCH_CHECK_TYPE(PyList_Check(args[0]) && PyList_Check(args[1]) &&
-                   PyList_GET_SIZE(args[0]) == PyList_GET_SIZE(args[1]),
-                   "one list of states for every parameter group");
+  TORCH_CHECK_TYPE(PyList_Check(args[0]), "parameter groups must be a list");
+  StateWalk states(args[1]);
   std::vector<incagg_adam_hyper> hyper;
   std::vector<AdamTensor> tensors;
   std::optional<at::Device> device;
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); i++) {
-    PyObject *group = PyList_GET_ITEM(args[0], i), *states = PyList_GET_ITEM(args[1], i);
+    PyObject *group = PyList_GET_ITEM(args[0], i);
     PyObject *params = entry(group, k_params), *betas = entry(group, k_betas);
-    TORCH_CHECK_TYPE(PyList_Check(params) && PyList_Check(states), "params must be a list");
-    TORCH_CHECK_VALUE(PyList_GET_SIZE(params) == PyList_GET_SIZE(states),
-                      "a group's parameters have changed since the optimizer was made");
+    TORCH_CHECK_TYPE(PyList_Check(params), "params must be a list");
     TORCH_CHECK_TYPE(PySequence_Check(betas) && PySequence_Size(betas) == 2, "betas must be a pair");
     THPObjectPtr b1(raised(PySequence_GetItem(betas, 0))), b2(raised(PySequence_GetItem(betas, 1)));
     hyper.push_back({to_double(entry(group, k_lr)), to_double(b1.get()), to_double(b2.get()),
                      to_double(entry(group, k_eps)), to_double(entry(group, k_decay))});
     for (Py_ssize_t j = 0; j < PyList_GET_SIZE(params); j++) {
-      const Tensor &p = to_tensor(PyList_GET_ITEM(params, j), "a parameter"), &g = p.grad();
+      PyObject *parameter = PyList_GET_ITEM(params, j);
+      const Tensor p = to_tensor(parameter, "a parameter"), g = p.grad();
       if (!device) device = p.device();
-      if (!g.defined()) continue;
-      PyObject *state = PyList_GET_ITEM(states, j);
+      if (!g.defined()) {
+        states.skip(parameter);
+        continue;
+      }
+      THPObjectPtr state(states.of(parameter));
       tensors.push_back({p, g, to_tensor(entry(state, k_m), "exp_avg"),
                          to_tensor(entry(state, k_v), "exp_avg_sq"),
                          to_tensor(entry(state, k_step), "step"), (int64_t)i});

@@ -112,8 +112,6 @@ class Adam:
                                  "exp_avg_sq": flat[sum(sizes) + off:sum(sizes) + off + p.numel()]
                                  .view_as(p)}
                 off += n
-        # (the same dicts by position: a lookup by tensor costs a fifth of a small step)
-        self._states = [[self.state[p] for p in group["params"]] for group in self.param_groups]
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         for group in self.param_groups:
@@ -130,7 +128,7 @@ class Adam:
         are read -- ``clip_grad_norm_`` and the step in two launches; ``p.grad`` itself stays as
         it is -- and the norm they had is returned (a scalar on the device)."""
         if max_norm is not None:
-            return ops.train_ops().adam_step_clipped(self.param_groups, self._states,
+            return ops.train_ops().adam_step_clipped(self.param_groups, self.state,
                                                      _max_norm(max_norm))
         return self._plain_step()
 

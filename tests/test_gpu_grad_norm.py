@@ -349,3 +349,74 @@ def test_clip_on_another_stream(optim, dev):
     torch.cuda.current_stream().wait_stream(side)
     assert abs(float(norm) - want) <= 2.0 ** -23 * want
     _check_clipped(before, [p.grad for p in params], 0.1 / (want + 1e-6))
+
+
+def _stepped(optim, shapes, change, clipped):
+    """Two steps with `change(optimizer, parameters)` between them; the parameters by name."""
+    dev = torch.device("cuda", 0)
+    gen = torch.Generator(device=dev).manual_seed(31)
+    params = [torch.randn(s, device=dev, generator=gen).requires_grad_() for s in shapes]
+    opt = optim.Adam([dict(params=params[:2]), dict(params=params[2:], lr=3e-3)], lr=1e-2)
+    for it in range(2):
+        for p in params:
+            p.grad = torch.randn(p.shape, device=dev, generator=gen)
+        if it == 1:
+            change(opt, params)
+        opt.step(max_norm=math.inf) if clipped else opt.step()
+    return params, opt
+
+
+def _replace_state(opt, params):
+    p = params[1]
+    opt.state[p] = {"step": torch.full((), 5.0, device=p.device),
+                    "exp_avg": torch.full_like(p, 0.5).detach(),
+                    "exp_avg_sq": torch.full_like(p, 0.25).detach()}
+
+
+def _reorder_parameters(opt, params):
+    for group in opt.param_groups:
+        group["params"].reverse()
+
+
+def _move_between_groups(opt, params):
+    opt.param_groups[1]["params"].insert(0, opt.param_groups[0]["params"].pop(0))
+
+
+def _reorder_states(opt, params):
+    opt.state[params[0]] = opt.state.pop(params[0])
+
+
+def _no_gradient(opt, params):
+    params[0].grad = params[3].grad = None
+
+
+@pytest.mark.parametrize("change", [
+    _replace_state, _reorder_parameters, _move_between_groups, _reorder_states, _no_gradient])
+def test_clipped_adam_finds_the_states_that_step_finds(optim, dev, change):
+    """Whatever was done to the state and the groups between two steps: with a bound that clips
+    nothing (a factor of exactly 1) the clipped step updates the same moments as step().  Both compute
+    the same formula in float32; step() evaluates 1 - 0.999^t in float32, off by up to 6e-5 of itself
+    at t = 1 and less later, half of that under the root: two moves of at most 3.2 lr = 0.032 differ by
+    less than 2 * 0.032 * 4e-5, the moments by a few roundings."""
+    shapes = [(40, 3), (40, 3), (40, 3), (7,), (40, 3)]
+    ours, opt = _stepped(optim, shapes, change, True)
+    ref, twin = _stepped(optim, shapes, change, False)
+    for p, r in zip(ours, ref):
+        assert float((p.detach() - r.detach()).abs().max()) <= 2 * 0.032 * 4e-5 + 2.0 ** -20
+        # (1 - beta from float32 betas: off by 2^-25 / 0.1 and by 2^-25 / 0.001, below 2^-15)
+        for key, part in (("exp_avg", 2.0 ** -20), ("exp_avg_sq", 2.0 ** -15), ("step", 0.0)):
+            a, b = opt.state[p][key], twin.state[r][key]
+            assert float((a - b).abs().max()) <= part * float(b.abs().max())
+
+
+def test_clipped_adam_refuses_a_parameter_without_state(optim, dev):
+    ours, opt = _stepped(optim, [(8,), (8,), (8,)], lambda *_: None, True)
+    kept = [p.detach().clone() for p in ours]
+    stranger = torch.zeros(8, device=dev, requires_grad=True)
+    stranger.grad = torch.ones(8, device=dev)
+    opt.param_groups[0]["params"][1] = stranger
+    for step in (lambda: opt.step(max_norm=1.0), opt.step):
+        with pytest.raises(KeyError):
+            step()
+    assert all(torch.equal(p.detach(), k) for p, k in zip(ours, kept))
+    assert float(stranger.detach().abs().sum()) == 0.0
