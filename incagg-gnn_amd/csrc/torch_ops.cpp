@@ -19,6 +19,8 @@
 #ifdef INCAGG_OPS_TRAIN
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
@@ -417,15 +419,18 @@ using torch::autograd::variable_list;
 
 // A backward pass that is recorded into a HIP graph must not meet a leaf whose accumulation node a
 // graph of the default stream keeps alive: autograd would tie the recording to that stream, which
-// ends the process.  An error instead, before anything of it runs.
-void check_recording(const Tensor &leaf) {
-  if (!leaf.requires_grad() || !leaf.is_leaf()) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+// ends the process.  An error instead, before anything of it runs.  Asked of the running node's edges,
+// which lead to the accumulation nodes of all its inputs, the bias (which is not saved) among them.
+void check_recording() {
+  const auto node = torch::autograd::get_current_node();
   if (!node) return;
-  const auto stream = node->stream();
-  TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(leaf.device().index()).id(),
-              "recording a backward pass while an earlier, eager graph of the same leaf is alive "
-              "(a loss or output that is still referenced): delete it before the recording begins");
+  for (const auto &edge : node->next_edges()) {
+    if (!dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get())) continue;
+    const auto stream = edge.function->stream();
+    TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(stream->device_index()).id(),
+                "recording a backward pass while an earlier, eager graph of the same leaf is alive "
+                "(a loss or output that is still referenced): delete it before the recording begins");
+  }
 }
 
 struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
@@ -448,10 +453,8 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
     variable_list out(7);
     {
       c10::DeviceGuard guard(x.device());
-      if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
-        check_recording(x);
-        check_recording(w);
-      }
+      if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+        check_recording();
     }
     {
       at::AutoGradMode no_graph(false);

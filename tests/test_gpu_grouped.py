@@ -712,3 +712,41 @@ def test_training_a_typed_network_end_to_end(nn, ops, dev):
     for p, r, s in zip(params, ref, start):
         moved = float((r.detach() - s).norm())
         assert moved > 0 and float((p.detach().double() - r.detach()).norm()) <= 0.02 * moved
+
+
+@pytest.mark.parametrize("trained", ["x", "weight", "bias"])
+def test_recorded_backward_of_one_leaf_beside_an_eager_graph(nn, ops, dev, trained):
+    """Whichever of the layer's inputs is the only one with a gradient: the recording is refused while
+    an eager graph of it lives, and runs once that graph is gone."""
+    gen, x, w, b, dy = _case(dev, 90, 3, 20, 12, F32, 41)
+    leaves = {"x": x, "weight": w, "bias": b}
+    leaf = leaves[trained].requires_grad_()
+    leaf.grad = torch.zeros_like(leaf)
+    groups = ops.group_rows(torch.arange(90, device=dev) % 3, 3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def step():
+        leaf.grad.zero_()
+        nn.grouped_linear(x, w, b, groups).square().sum().backward()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    alive = nn.grouped_linear(x, w, b, groups).sum()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph, stream=side):
+            step()
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for it in range(3):
+        with torch.no_grad():
+            leaf.copy_(torch.randn(leaf.shape, device=dev, generator=gen))
+        graph.replay()
+        got = leaf.grad.clone()
+        step()
+        torch.cuda.synchronize()
+        assert float(got.abs().sum()) > 0 and torch.equal(got, leaf.grad)
