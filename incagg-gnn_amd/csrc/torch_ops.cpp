@@ -382,14 +382,17 @@ struct Groups {
 Tensor grouped_gemm(const Tensor &x_in, const Tensor &w_in, bool trans_w, const Tensor &bias_in,
                     const Groups &groups, int64_t pitch) {
   const Tensor x = plain_rows(x_in);
-  const bool plain = w_in.stride(2) == 1 && w_in.stride(1) >= w_in.size(2);
-  const Tensor w = plain ? w_in : w_in.contiguous();
+  // (the stride of a dimension of one says nothing, and contiguous() leaves it as it is)
+  const bool unit = w_in.size(2) <= 1 || w_in.stride(2) == 1;
+  const bool apart = w_in.size(1) <= 1 || w_in.stride(1) >= w_in.size(2);
+  const Tensor w = unit && apart ? w_in : w_in.contiguous();
+  const int64_t ldw = w.size(1) > 1 ? w.stride(1) : w.size(2);
   const Tensor bias = bias_in.defined() ? plain_rows(bias_in) : bias_in;
   const int64_t rows = x.size(0), k = x.size(1), n = w.size(trans_w ? 1 : 2);
   Tensor y = rows_empty(rows, n, pitch, x);
   c10::DeviceGuard guard(x.device());
   check_status(incagg_grouped_gemm(
-      ptr_or_null<void>(x), pitch_of(x), w.data_ptr(), w.stride(1), w.stride(0), trans_w ? 1 : 0,
+      ptr_or_null<void>(x), pitch_of(x), w.data_ptr(), ldw, w.stride(0), trans_w ? 1 : 0,
       bias.defined() ? bias.data_ptr() : nullptr, bias.defined() ? pitch_of(bias) : 0,
       groups.ptr_data(), groups.order_data(), groups.count(), rows, k, n, (int)element_code(x),
       const_cast<void *>(ptr_or_null<void>(y)), pitch_of(y), current_stream(x.device())));

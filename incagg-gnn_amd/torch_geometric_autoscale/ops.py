@@ -885,10 +885,10 @@ def grouped_gemm(x: Tensor, w: Tensor, groups: RowGroups, trans_w: bool = False,
     if w.device != dev or (bias is not None and bias.device != dev):
         raise ValueError("x, w and bias must be on one device")
     x = _plain_rows(x)
-    w_group, ldw, unit = w.stride()
-    if unit != 1 or ldw < w.shape[2] or w_group < 0:
+    # (the stride of a dimension of one says nothing, and contiguous() leaves it as it is)
+    if (w.shape[2] > 1 and w.stride(2) != 1) or (w.shape[1] > 1 and w.stride(1) < w.shape[2]):
         w = w.contiguous()
-        w_group, ldw, _ = w.stride()
+    w_group, ldw = w.stride(0), w.stride(1) if w.shape[1] > 1 else w.shape[2]
     ld_bias = 0
     if bias is not None:
         if tuple(bias.shape) != (n_groups, n):

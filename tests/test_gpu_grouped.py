@@ -750,3 +750,34 @@ def test_recorded_backward_of_one_leaf_beside_an_eager_graph(nn, ops, dev, train
         step()
         torch.cuda.synchronize()
         assert float(got.abs().sum()) > 0 and torch.equal(got, leaf.grad)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n_groups", [1, 3])
+@pytest.mark.parametrize("rows", [40, 700])
+def test_weights_with_a_dimension_of_one(nn, ops, dev, dtype, n_groups, rows):
+    """Transposed views whose dimension of one has a stride that means nothing, and that count as
+    contiguous: one output per kind, one input."""
+    gen, x, _, _, dy = _case(dev, rows, n_groups, 40, 24, dtype, 43)
+    ids = _ids("ragged", rows, n_groups, dev, gen)
+    groups = ops.group_rows(ids, n_groups)
+    for k, n in ((40, 1), (1, 24), (1, 1)):
+        xk, dyn = x[:, :k], dy[:, :n]
+        plain = torch.randn(n_groups, n, k, device=dev, generator=gen).to(dtype)
+        flip = plain.transpose(1, 2).contiguous().transpose(1, 2)         # [G, n, k] out of [G, k, n]
+        odd = torch.as_strided(flip, flip.shape, [flip.stride(0)] + [
+            3 if size == 1 else stride for size, stride in zip(flip.shape[1:], flip.stride()[1:])])
+        for w in (flip, odd):
+            assert torch.equal(w, plain)
+            _close(ops.grouped_gemm(xk, w, groups, trans_w=True), *_rows64(xk, plain, None, ids, True),
+                   k, dtype)
+            _close(ops.grouped_gemm(dyn, w, groups), *_rows64(dyn, plain, None, ids, False), n, dtype)
+            wt = w.transpose(1, 2)                                        # [G, k, n]
+            _close(ops.grouped_gemm(xk, wt, groups), *_rows64(xk, plain, None, ids, True), k, dtype)
+            xl, wl = xk.detach().clone().requires_grad_(), w.detach().requires_grad_()
+            y = nn.grouped_linear(xl, wl, None, groups)
+            _close(y.detach(), *_rows64(xk, plain, None, ids, True), k, dtype)
+            dx, dw = torch.autograd.grad(y, [xl, wl], dyn)
+            _close(dx, *_rows64(dyn, plain, None, ids, False), n, dtype)
+            d, mag, _, _, count = _tn64(dyn, xk, ids, n_groups)
+            _close(dw, d, mag, count.view(-1, 1, 1), dtype)
