@@ -330,14 +330,21 @@ __device__ inline void multiply(const unsigned short *rows, const unsigned short
   }
 }
 
-template <int MI, int NJ> __device__ inline bool all_finite(const f4 (&acc)[MI][NJ]) {
+// Whether this lane's results are all finite: of the rows that keeps(i) names (of blocks i) and the
+// first `columns` columns from its own first on.  What is not stored may come from any row or column
+// of the operands, and does not count.
+template <int MI, int NJ, typename Keeps>
+__device__ inline bool all_finite(const f4 (&acc)[MI][NJ], int columns, Keeps &&keeps) {
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < MI; i++)
+  for (int i = 0; i < MI; i++) {
+    const int count = keeps(i) ? columns : 0;
 #pragma unroll
     for (int j = 0; j < NJ; j++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) s = fmaf(acc[i][j][e], 0.f, s);     // NaN once one is not finite
+      for (int e = 0; e < 4; e++)         // NaN once one is not finite
+        s = fmaf(16 * j + e < count ? acc[i][j][e] : 0.f, 0.f, s);
+  }
   return s == 0.f;
 }
 
@@ -626,7 +633,11 @@ void grouped_rows_kernel(const GroupedArgs a) {
   const RowsOut<D> out{a, g};
   const int lane = tid & 63;
   if constexpr (D == INCAGG_DTYPE_F32) {
-    if (g < a.n_groups && __syncthreads_or(!all_finite(acc))) {
+    const int columns = a.n - (n0 + col0 + 4 * (lane >> 4));
+    const bool finite = all_finite(acc, columns, [&](int i) __attribute__((always_inline)) {
+      return row_ids[row0 + 16 * i + (lane & 15)] >= 0;
+    });
+    if (g < a.n_groups && __syncthreads_or(!finite)) {
       // (a value that does not split, or a result out of range: plain multiply-adds)
       for (int ij = 0; ij < MI * NJ; ij++) {
         const int id = row_ids[row0 + 16 * (ij / NJ) + (lane & 15)];
@@ -806,7 +817,12 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
   }
   const TnOut<D> out{t, g, seg, whole};
   bool again = false;
-  if constexpr (D == INCAGG_DTYPE_F32) again = __syncthreads_or(!all_finite(acc));
+  if constexpr (D == INCAGG_DTYPE_F32) {
+    const int columns = t.n - (n0 + col0 + 4 * (lane >> 4)), left = t.m - (m0 + row0 + (lane & 15));
+    again = __syncthreads_or(!all_finite(acc, columns, [&](int i) __attribute__((always_inline)) {
+      return 16 * i < left;
+    }));
+  }
   if (again) {          // (a value that does not split, or a result out of range)
     for (int ij = 0; ij < MI * NJ; ij++) {
       const int m = m0 + row0 + 16 * (ij / NJ) + (lane & 15);

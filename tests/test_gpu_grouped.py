@@ -781,3 +781,43 @@ def test_weights_with_a_dimension_of_one(nn, ops, dev, dtype, n_groups, rows):
             _close(dx, *_rows64(dyn, plain, None, ids, False), n, dtype)
             d, mag, _, _, count = _tn64(dyn, xk, ids, n_groups)
             _close(dw, d, mag, count.view(-1, 1, 1), dtype)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -3.4e38])
+@pytest.mark.parametrize("rows,n_groups", [(60, 5), (700, 5), (200_000, 3)])
+def test_rows_and_columns_of_others_leave_no_trace(ops, dev, rows, n_groups, bad):
+    """float32 tiles are filled up with rows and columns that belong to others.  One that is not
+    finite (or rounds to an infinity in 16 bits) changes no bit of anything it does not belong to."""
+    k, n = 129, 129
+    gen, x, w, b, dy = _case(dev, rows, n_groups, k, n, F32, 47)
+    ids = _ids("random", rows, n_groups, dev, gen)
+    ids[0] = -1                                  # the first row belongs to no group
+    x[0], dy[0] = 0, 0
+    groups = ops.group_rows(ids, n_groups)
+    wt = w.transpose(1, 2).contiguous()                                   # [G, k, n]
+
+    def results():
+        dw, db = ops.grouped_tn(dy, x, groups, column_sums=True)
+        return (ops.grouped_gemm(x, w, groups, trans_w=True, bias=b), ops.grouped_gemm(x, wt, groups),
+                ops.grouped_gemm(dy, w, groups), dw, db, ops.grouped_tn(x, dy, groups))
+    clean = results()
+    x[0], dy[0] = bad, bad
+    assert all(torch.equal(a, c) for a, c in zip(results(), clean))
+    # a column of the operands: the tile of the last column is filled up with the ones in front of it,
+    # which belong to another tile
+    x[0], dy[0] = 0, 0
+    last = slice(128, None)
+    for at in (126, 127):
+        keep = [(t, t.clone()) for t in (x, dy, w, wt)]
+        x[:, at], dy[:, at] = bad, bad
+        dw, db = ops.grouped_tn(dy, x, groups, column_sums=True)
+        assert torch.equal(dw[:, last, last], clean[3][:, last, last])
+        assert torch.equal(db[:, last], clean[4][:, last])
+        assert torch.equal(ops.grouped_tn(x, dy, groups)[:, last, last], clean[5][:, last, last])
+        for t, old in keep:
+            t.copy_(old)
+        wt[:, :, at], w[:, :, at] = bad, bad
+        assert torch.equal(ops.grouped_gemm(x, wt, groups)[:, last], clean[1][:, last])
+        assert torch.equal(ops.grouped_gemm(dy, w, groups)[:, last], clean[2][:, last])
+        for t, old in keep:
+            t.copy_(old)
