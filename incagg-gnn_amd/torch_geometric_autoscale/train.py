@@ -64,8 +64,9 @@ def mini_train(model, loader, criterion, optimizer, max_steps, grad_norm=None, e
     after its first (eager) execution and replayed whenever the batch comes up again."""
     model.train()
     total_loss, total_examples = 0.0, 0     # the loss sum stays on the device until the end
-    # (the norm is taken over the model's parameters: the optimizer has to hold the same ones)
-    clip_in_step = isinstance(optimizer, Adam) and (
+    # (the norm is taken over the model's parameters: the optimizer has to hold the same ones, and
+    # its step() has to be the one that clips)
+    clip_in_step = getattr(optimizer.step, "__func__", None) is Adam.step and (
         {id(p) for g in optimizer.param_groups for p in g["params"]}
         == {id(p) for p in model.parameters()})
     clip = (clip_grad_norm_ if torch.device(model.device).type == "cuda"
