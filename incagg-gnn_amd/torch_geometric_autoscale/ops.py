@@ -736,6 +736,11 @@ def softmax_cross_entropy(logits: Tensor, labels: Tensor) -> Tensor:
 
 # --------------------------------------------------------------------------- rows of several kinds
 _train_ops = None
+TRAIN_OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_train_ops.so")
+
+
+def train_ops_built() -> bool:
+    return _train_ops is not None or os.path.isfile(TRAIN_OPS_PATH)
 
 
 def train_ops():
@@ -743,10 +748,9 @@ def train_ops():
     Python would take longer than their kernels."""
     global _train_ops
     if _train_ops is None:
-        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_train_ops.so")
-        if not os.path.isfile(path):
+        if not train_ops_built():
             raise _lib.IncAggLibraryError(
-                f"{path} not found: build it with `python incagg-gnn_amd/csrc/build_torch_ops.py` "
+                f"{TRAIN_OPS_PATH} not found: build it with `python incagg-gnn_amd/csrc/build_torch_ops.py` "
                 "(there is no fallback implementation)")
         _train_ops = importlib.import_module("._train_ops", __package__)
     return _train_ops

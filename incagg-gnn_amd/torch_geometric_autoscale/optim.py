@@ -66,6 +66,18 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     return torch.zeros(()) if norm is None else norm
 
 
+def clips(parameters: Union[Tensor, Iterable[Tensor]]) -> bool:
+    """Whether :func:`clip_grad_norm_` takes these gradients (``torch.nn.utils.clip_grad_norm_`` takes
+    more): they are dense, of float32, bfloat16 or float16, on one GPU, and none is listed twice; and
+    `_train_ops.so` is built."""
+    grads = [g for g in [p.grad for p in _list(parameters)] if g is not None]
+    return (ops.train_ops_built()
+            and all(g.is_cuda and g.dtype in ops.DTYPE_CODE and g.layout == torch.strided
+                    and g.device == grads[0].device for g in grads)
+            and len({g.data_ptr() for g in grads if g.numel()})
+            == sum(1 for g in grads if g.numel()))
+
+
 class Adam:
     """Subset of ``torch.optim.Adam``: ``params`` (tensors or group dicts with their own ``lr`` /
     ``weight_decay``, as main.py:160-165 builds them), ``lr``, ``betas``, ``eps``,

@@ -29,7 +29,7 @@ from .data import gcn_norm, get_data
 from .loader import DeviceSubgraphLoader, EvalSubgraphLoader, SubgraphLoader
 from .metis import load_partition, metis, permute
 from .nn import CrossEntropyLoss
-from .optim import Adam, clip_grad_norm_
+from .optim import Adam, clip_grad_norm_, clips
 from .utils import compute_micro_f1, dropout
 
 log = logging.getLogger("incagg.train")
@@ -61,7 +61,11 @@ def mini_train(model, loader, criterion, optimizer, max_steps, grad_norm=None, e
     ``graphs`` (a ``graphs.StepGraphs``): with a loader that keeps its batch objects
     (``static_batches``) and no edge dropout, the step of a batch -- forward, loss, backward,
     gradient clipping, optimizer step, loss bookkeeping -- is recorded into a HIP graph right
-    after its first (eager) execution and replayed whenever the batch comes up again."""
+    after its first (eager) execution and replayed whenever the batch comes up again.
+
+    ``grad_norm`` clips with the kernels of ``optim`` where they take the gradients
+    (``optim.clips``), with ``torch.nn.utils.clip_grad_norm_`` otherwise.  An ``optim.Adam`` over the
+    model's parameters clips them as it reads them: ``p.grad`` stays unscaled then."""
     model.train()
     total_loss, total_examples = 0.0, 0     # the loss sum stays on the device until the end
     # (the norm is taken over the model's parameters: the optimizer has to hold the same ones, and
@@ -69,8 +73,6 @@ def mini_train(model, loader, criterion, optimizer, max_steps, grad_norm=None, e
     clip_in_step = getattr(optimizer.step, "__func__", None) is Adam.step and (
         {id(p) for g in optimizer.param_groups for p in g["params"]}
         == {id(p) for p in model.parameters()})
-    clip = (clip_grad_norm_ if torch.device(model.device).type == "cuda"
-            else torch.nn.utils.clip_grad_norm_)
     replayable = (graphs is not None and getattr(loader, "static_batches", False)
                   and not edge_dropout and torch.device(model.device).type == "cuda")
     if replayable:
@@ -110,10 +112,13 @@ def mini_train(model, loader, criterion, optimizer, max_steps, grad_norm=None, e
             loss.backward()
             if grad_norm is None:
                 optimizer.step()
+            elif not clips(model.parameters()):     # on the host, float64, sparse, ...
+                torch.nn.utils.clip_grad_norm_(model.parameters(), grad_norm)
+                optimizer.step()
             elif clip_in_step:          # clipped as the optimizer reads them
                 optimizer.step(max_norm=grad_norm)
             else:
-                clip(model.parameters(), grad_norm)
+                clip_grad_norm_(model.parameters(), grad_norm)
                 optimizer.step()
             return loss.detach()
 

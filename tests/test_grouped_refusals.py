@@ -148,3 +148,17 @@ def test_workspace_bounds_cover_the_launches(L):
         need = sum(min(1024, sum(-(-n // 8192) for n in live[i:i + 128]))
                    for i in range(0, len(live), 128))
         assert L.incagg_grad_norm_ws_doubles(len(sizes), sum(sizes)) >= need
+
+
+def test_a_missing_training_module_fails_loudly(monkeypatch):
+    from torch_geometric_autoscale import _lib, ops, optim
+    assert ops.train_ops_built()
+    monkeypatch.setattr(ops, "_train_ops", None)
+    monkeypatch.setattr(ops, "TRAIN_OPS_PATH", "/nonexistent/_train_ops.so")
+    assert not ops.train_ops_built()
+    p = torch.nn.Parameter(torch.zeros(3))
+    for call in (ops.train_ops, lambda: optim.clip_grad_norm_(p, 1.0), lambda: optim.grad_norm(p),
+                 lambda: ops.group_rows(torch.zeros(3, dtype=torch.int64), 2)):
+        with pytest.raises(_lib.IncAggLibraryError):
+            call()
+    assert not optim.clips([p])
