@@ -12,14 +12,15 @@
 //
 // Matrix cores.  Everything runs on v_mfma_f32_16x16x32_{bf16,f16}: 16 times the rate of the
 // float32 instruction.  bfloat16 and float16 operands go in as they are.  A float32 value goes in
-// as three bfloat16 values, x = h + m + l, each the nearest to what the ones before it leave:
-// |x - h - m - l| <= 2^-27 |x|.  A product of two of them is hh + hm + mh + mm + hl + lh; what is
-// left out (ml, lm, ll and the two remainders) is below 2^-25 of the product, half a float32
-// rounding, and the sums are float32 as ever.  Six instructions against sixteen.  (A value under
-// 2^-110 keeps an absolute error of 2^-134, bfloat16's smallest step, in place of the relative one.)
-// Infinities, NaNs and values that round to infinity as bfloat16 do not split: their parts are
-// not finite, so every result they enter is not, and a tile with such a result is computed again
-// with plain float32 multiply-adds.
+// as three bfloat16 values, 2^16 x = h + m + l, each the nearest to what the ones before it leave.
+// The sum is exact: 3 x 8 bits, and the last bit of the smallest float32 value, 2^-149, times 2^16 is
+// bfloat16's own last bit (without the factor, values under 2^-110 lose bits: errors of 3e-4 for 1e37 x
+// 1e-37).  A product of two of them is hh + hm + mh + mm + hl + lh; what is left out, ml + lm + ll, is
+// at most 2^-24 of the product (|m| <= 2^-8, |l| <= 2^-17 of a value in [1, 2)), one float32 rounding,
+// and the sums are float32 as ever, scaled by 2^-32 at their end.  Six instructions against sixteen.
+// Infinities, NaNs, values from 2^112 on and sums from 2^96 on do not go through: their parts or sums
+// are not finite, and a tile with such a result is computed again with plain float32 multiply-adds
+// (a loop over k for each of its results).
 //
 // LDS holds K-contiguous tiles, [row][BK], one per part of the split, in 16-byte pieces that are
 // permuted within 128 bytes so that both the fragment reads and the writes spread over the banks.
@@ -91,12 +92,13 @@ template <int BK> __device__ inline int piece_at(int row, int chunk) {
 }
 
 // Eight float32 values along k of one row: into the three parts of its tile (PLANE values apart).
+constexpr float kSplitScale = 0x1p16f, kSplitUnscale = 0x1p-32f;      // of a value, of a sum of products
 template <int PLANE>
 __device__ inline void put_split(unsigned short *tile, int at, const float (&v)[8]) {
   u4 h, m, l;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    f2 x = {v[2 * i], v[2 * i + 1]};
+    f2 x = {v[2 * i] * kSplitScale, v[2 * i + 1] * kSplitScale};
     const unsigned hb = __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf2));
     x.x -= __uint_as_float(hb << 16);
     x.y -= __uint_as_float(hb & 0xffff0000u);
@@ -346,6 +348,16 @@ __device__ inline bool all_finite(const f4 (&acc)[MI][NJ], int columns, Keeps &&
         s = fmaf(16 * j + e < count ? acc[i][j][e] : 0.f, 0.f, s);
   }
   return s == 0.f;
+}
+
+// Sums of products of split values, back from their scale.
+template <int MI, int NJ> __device__ inline void unscale(f4 (&acc)[MI][NJ]) {
+#pragma unroll
+  for (int i = 0; i < MI; i++)
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[i][j][e] *= kSplitUnscale;
 }
 
 // Four neighbouring results of a row, rounded to their type.
@@ -657,6 +669,7 @@ void grouped_rows_kernel(const GroupedArgs a) {
       }
       return;
     }
+    unscale(acc);
   }
   __syncthreads();                       // (the tiles are read no more)
   out.put_all(acc, row_ids + row0, n0 + col0, tiles + wave * kRowScratch<D, NJ>);
@@ -840,6 +853,7 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
       out.put(m, n, v);
     }
   } else {
+    if constexpr (D == INCAGG_DTYPE_F32) unscale(acc);
     __syncthreads();                     // (the tiles are read no more)
     out.put_all(acc, m0 + row0, n0 + col0, tiles + wave * kRowScratch<INCAGG_DTYPE_F32, NJ>);
   }

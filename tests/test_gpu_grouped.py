@@ -821,3 +821,46 @@ def test_rows_and_columns_of_others_leave_no_trace(ops, dev, rows, n_groups, bad
         assert torch.equal(ops.grouped_gemm(dy, w, groups)[:, last], clean[2][:, last])
         for t, old in keep:
             t.copy_(old)
+
+
+@pytest.mark.parametrize("rows", [20, 700])
+@pytest.mark.parametrize("power", [-140, -126, -118, -110, -100, 60, 100, 111, 113, 120])
+def test_float32_over_its_whole_range(ops, dev, rows, power):
+    """Factors around 2^power and 2^-power (at most 2^122): products near 1, so the tolerance is that of
+    any float32 sum, whatever parts the factors are taken into."""
+    n_groups, k, n = 3, 64, 48
+    gen, x, w, b, dy = _case(dev, rows, n_groups, k, n, F32, 53)
+    ids = _ids("random", rows, n_groups, dev, gen)
+    groups = ops.group_rows(ids, n_groups)
+    other = min(-power, 122)
+
+    def at(t, p):           # (in two steps: 2^-140 is no normal float32)
+        return t * 2.0 ** (p // 2) * 2.0 ** (p - p // 2)
+    xs, ws, dys, xo = at(x, power), at(w, other), at(dy, power), at(x, other)
+    _close(ops.grouped_gemm(xs, ws, groups, trans_w=True, bias=b), *_rows64(xs, ws, b, ids, True), k + 1,
+           F32)
+    _close(ops.grouped_gemm(dys, ws, groups), *_rows64(dys, ws, None, ids, False), n, F32)
+    dw, db = ops.grouped_tn(dys, xo, groups, column_sums=True)
+    d, mag, s, smag, count = _tn64(dys, xo, ids, n_groups)
+    _close(dw, d, mag, count.view(-1, 1, 1), F32)
+    _close(db, s, smag, count.view(-1, 1), F32)
+
+
+@pytest.mark.parametrize("power", [-40, -60, -66, -72, 40, 46, 50, 60])
+def test_float32_results_over_their_whole_range(ops, dev, power):
+    """Both factors around 2^power: results down to where float32 loses them (2^-149 in the tolerance:
+    half a step of the smallest values, and one more for a partial sum), and up to 2^124."""
+    rows, n_groups, k, n = 300, 3, 64, 48
+    gen, x, w, b, dy = _case(dev, rows, n_groups, k, n, F32, 59)
+    ids = _ids("random", rows, n_groups, dev, gen)
+    groups = ops.group_rows(ids, n_groups)
+    x, w, dy = x * 2.0 ** power, w * 2.0 ** power, dy * 2.0 ** power
+
+    def close(got, want, mag, length):
+        tol = (length + 8) * 2.0 ** -23 * mag + HALF_STEP[F32] * want.abs() + 2 * 2.0 ** -149
+        assert bool(((got.double() - want).abs() <= tol).all())
+    close(ops.grouped_gemm(x, w, groups, trans_w=True), *_rows64(x, w, None, ids, True), k)
+    close(ops.grouped_gemm(dy, w, groups), *_rows64(dy, w, None, ids, False), n)
+    dw = ops.grouped_tn(dy, x, groups)
+    d, mag, _, _, count = _tn64(dy, x, ids, n_groups)
+    close(dw, d, mag, count.view(-1, 1, 1))
