@@ -898,15 +898,10 @@ __device__ const u4 g_zeros = {0u, 0u, 0u, 0u};
 
 // The instruction has no result register, and its address registers are read when it issues.  (As
 // a builtin, the compiler makes the next LDS read wait for it, whichever buffer that one reads.)
-// m0: where in LDS lane 0's piece goes.  The compiler allocates it to nothing, which it remarks on when
-// m0 is named as overwritten; naming it keeps a value that it puts there itself from being used behind.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
+// m0: where in LDS lane 0's piece goes; put there by the compiler, which then knows what m0 holds.
 __device__ inline void load_to_lds(const void *src, unsigned lds_byte) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :: "s"(lds_byte), "v"(src) : "memory", "m0");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "{m0}"(lds_byte), "v"(src) : "memory");
 }
-#pragma clang diagnostic pop
 
 // Waits for this wave's loads into LDS; with a barrier behind it, for everybody's.
 __device__ inline void loads_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
