@@ -17,10 +17,14 @@
 // per element against 2 or 4 bytes of memory traffic).  coef is rounded to float32 once; a scaled
 // value is rounded once, to its own type.
 //
-// Bound by memory once there is enough of it.  200 M elements in 300 tensors of three types: norm 107
-// us (read at 5.6 TB/s), norm and scaling 258 us; Adam with clipping over 64 M parameters 412 us (28
-// bytes each at 5.1 TB/s: 351 us, and the norm in front of it).  Small ones are two launches: 10
-// tensors of 110 k elements 12.5 us, Adam over 20 tensors of 1.1 M 15.6 us, most of both on the host.
+// Bound by memory once there is enough of it: the norm of 200 M bfloat16 elements (400 MB) in one
+// tensor takes 72 us (5.5 TB/s), of 100 M float32 ones 70 us.  In 300 tensors it takes 87 us (4.6 TB/s):
+// three launches, the next of which starts when the last workgroup of the one before has ended.
+// Clipping those 300 (nearly all bfloat16, some short float32) takes 265 us where they are scaled (1.2
+// GB, 4.5 TB/s) and 110 us where they are not: three more launches, which add up the partials and end.
+// Adam with clipping over 64 M parameters 412 us (28 bytes each at 5.1 TB/s: 351 us, and the norm in
+// front of it).  Small ones are two launches: 10 tensors of 110 k elements 11-13 us, Adam over 20
+// tensors of 1.1 M 14.5-17 us, most of both on the host.
 #include "common.h"
 
 #include <hip/hip_bf16.h>

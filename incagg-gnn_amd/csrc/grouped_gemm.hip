@@ -18,9 +18,14 @@
 // 1e-37).  A product of two of them is hh + hm + mh + mm + hl + lh; what is left out, ml + lm + ll, is
 // at most 2^-24 of the product (|m| <= 2^-8, |l| <= 2^-17 of a value in [1, 2)), one float32 rounding,
 // and the sums are float32 as ever, scaled by 2^-32 at their end.  Six instructions against sixteen.
+// (The scaling costs 2 %: 128064 x 100 -> 256 77.0 / 78.8 us without / with.  The float32 figures at the
+// choices of tiles below were taken without it, on both sides.)
 // Infinities, NaNs, values from 2^112 on and sums from 2^96 on do not go through: their parts or sums
-// are not finite, and a tile with such a result is computed again with plain float32 multiply-adds
-// (a loop over k for each of its results).
+// are not finite, and a tile with such a result is computed again with plain float32 multiply-adds, a
+// loop over k for each of its results, over the rows of its segment in the weight gradient.  Right, but
+// slow: one row of NaNs takes 128064 x 100 -> 256 from 76 to 339 us and its weight gradient from 97 to
+// 2100, 200000 x 512 -> 256 in one group from 380 us to 4 ms and from 390 us to 17 ms; one in every 16
+// rows, the former from 380 us to 49 ms.
 //
 // LDS holds K-contiguous tiles, [row][BK], one per part of the split, in 16-byte pieces that are
 // permuted within 128 bytes so that both the fragment reads and the writes spread over the banks.
@@ -884,8 +889,9 @@ __global__ __launch_bounds__(256, 2) void grouped_tn_kernel(const TnArgs t) {
 //     k % 4 + 4 (k / 8 % 2).  A fragment is two transposing reads (ds_read_b64_tr_b16: 16 lanes
 //     name 4 rows x 16 columns, lane i gets column i): the 32 lanes of a read phase touch rows
 //     0..3 and 8..11 of a 16-row block, which f spreads over all 64 banks.
-// The permutation is applied where it is free, to the address each lane loads from (no bank
-// conflicts in either form, by the counters).  What lies past the end of the reduction is loaded
+// The permutation is applied where it is free, to the address each lane loads from (bank conflicts
+// take 4 to 7 % of the LDS cycles, those of the results' way out, put_rows, included).  What lies past
+// the end of the reduction is loaded
 // from 16 bytes of zeros.
 //
 // Two buffers and one barrier a chunk.  Fragments are read AHEAD row blocks before they are
@@ -1292,7 +1298,10 @@ static bool pieces(const void *p, int64_t ld, int64_t width) {
 //                128    35.8   36.8   37.3   40.2   58.0   60.3   92.8
 //     float32     16    21.0   24.7   33.7   49.0   82.0    150    289
 //                 64    31.5   30.0   30.9   39.4   47.2   66.3    113
-//                128    44.0   43.1   43.6   44.2   46.9   75.8    120     (8192 rows: 941 / 881)
+//               128    44.0   43.1   43.6   44.2   46.9   75.8    120     (8192 rows: 941 / 881)
+// The average is all the host knows: it counts groups without a row, so many groups of which few are
+// used get tiles that are too low.  32768 rows in 8 groups of 8 / 64 / 512 / 2048, 512 -> 512: bfloat16
+// 36 / 35 / 61 / 286 us, float32 116 / 123 / 202 / 673.
 template <int D> static int launch_rows(GroupedArgs &a, bool trans_w, hipStream_t s) {
   constexpr bool F32 = D == INCAGG_DTYPE_F32;
   constexpr int STAGES = F32 ? 1 : 2;

@@ -552,7 +552,9 @@ def grouped_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], groups: "o
                    gathered: bool = False) -> Tensor:
     """``x[i] @ weight[g]^T + bias[g]`` for every row ``i``, ``g`` its group (``groups``:
     ops.group_rows / ops.groups_from_ptr); ``weight``: [n_groups, out, in], ``bias``:
-    [n_groups, out] or ``None``.  Rows of no group give zeros, and get zero gradients.
+    [n_groups, out] or ``None``.  Rows of no group give zeros, and get zero gradients.  float32
+    infinities and NaNs, values from 2^112 on and sums from 2^96 on are right but slow (their tile of
+    the result is computed again without the matrix cores).
     ``gathered``: a float32 result gets the row pitch an aggregation wants of its source."""
     pitch = dx_pitch = 0
     if gathered and x.dtype == torch.float32 and x.dim() == 2 and weight.dim() == 3:

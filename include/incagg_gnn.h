@@ -407,8 +407,9 @@ int incagg_group_ptr(const void *in, int in_is_64, int64_t n_groups, int64_t row
  *   y[i, :n] = x[i, :k] @ W_g + bias[g, :n]     g the group of row i; W_g = w[g] ([k, n]) or
  *                                               w[g]^T (w[g]: [n, k], trans_w); bias optional
  * and y[i] = 0 for rows of no group.  w_group: elements between the weights of two groups.  x, w,
- * bias and y are of one dtype; sums are held in fp32 and rounded once.  A row number outside
- * [0, rows) in order is skipped and reported. */
+ * bias and y are of one dtype; sums are held in fp32 and rounded once.  (fp32 results that are not
+ * finite, values from 2^112 on and sums from 2^96 on take a slow path, a tile at a time.)  A row number
+ * outside [0, rows) in order is skipped and reported. */
 int incagg_grouped_gemm(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t w_group,
                         int trans_w, const void *bias, int64_t ld_bias, const int32_t *ptr,
                         const int32_t *order, int64_t n_groups, int64_t rows, int64_t k, int64_t n,
