@@ -420,3 +420,30 @@ def test_clipped_adam_refuses_a_parameter_without_state(optim, dev):
             step()
     assert all(torch.equal(p.detach(), k) for p, k in zip(ours, kept))
     assert float(stranger.detach().abs().sum()) == 0.0
+
+
+def test_clipped_adam_with_more_groups_than_a_launch_takes(optim, dev):
+    """Twenty groups, each with hyperparameters of its own (a launch holds eight), first step: a move of
+    at most lr (a factor of sqrt(1 - b2) / (1 - b1) more for the moments' weights) in under ten float32
+    operations, and the rounding of p."""
+    gen = torch.Generator(device=dev).manual_seed(61)
+    ours = [torch.randn(33 + i, device=dev, generator=gen).requires_grad_() for i in range(40)]
+    hyper = [dict(lr=1e-3 * (i + 1), betas=(0.9 - 0.01 * i, 0.999 - 0.01 * i), eps=1e-8,
+                  weight_decay=1e-3 * (i % 3)) for i in range(20)]
+    opt = optim.Adam([dict(params=ours[2 * i:2 * i + 2], **h) for i, h in enumerate(hyper)])
+    for p in ours:
+        p.grad = torch.randn(p.shape, device=dev, generator=gen)
+    start = [p.detach().double() for p in ours]
+    want = _norm64([p.grad for p in ours], 2.0)
+    norm = opt.step(max_norm=0.5 * want)
+    assert abs(float(norm) - want) <= 2.0 ** -23 * want
+    coef = 0.5 * want / (want + 1e-6)
+    for j, (p, s) in enumerate(zip(ours, start)):
+        h = hyper[j // 2]
+        zero = torch.zeros_like(s)
+        new, m, v = _adam64(s, p.grad.double(), zero, zero, 1, coef, h["lr"], *h["betas"], h["eps"],
+                            h["weight_decay"])
+        tol = 16 * 2.0 ** -24 * h["lr"] * 3.2 + 2.0 ** -24 * new.abs()
+        assert bool(((p.detach().double() - new).abs() <= tol).all())
+        assert bool(((opt.state[p]["exp_avg"].double() - m).abs() <= 2.0 ** -21 * m.abs()).all())
+        assert bool(((opt.state[p]["exp_avg_sq"].double() - v).abs() <= 2.0 ** -21 * v.abs()).all())
