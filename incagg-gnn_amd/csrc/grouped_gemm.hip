@@ -1298,7 +1298,7 @@ static bool pieces(const void *p, int64_t ld, int64_t width) {
 //                128    35.8   36.8   37.3   40.2   58.0   60.3   92.8
 //     float32     16    21.0   24.7   33.7   49.0   82.0    150    289
 //                 64    31.5   30.0   30.9   39.4   47.2   66.3    113
-//               128    44.0   43.1   43.6   44.2   46.9   75.8    120     (8192 rows: 941 / 881)
+//                128    44.0   43.1   43.6   44.2   46.9   75.8    120     (8192 rows: 941 / 881)
 // The average is all the host knows: it counts groups without a row, so many groups of which few are
 // used get tiles that are too low.  32768 rows in 8 groups of 8 / 64 / 512 / 2048, 512 -> 512: bfloat16
 // 36 / 35 / 61 / 286 us, float32 116 / 123 / 202 / 673.

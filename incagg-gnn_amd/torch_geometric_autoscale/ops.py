@@ -750,8 +750,8 @@ def train_ops():
     if _train_ops is None:
         if not train_ops_built():
             raise _lib.IncAggLibraryError(
-                f"{TRAIN_OPS_PATH} not found: build it with `python incagg-gnn_amd/csrc/build_torch_ops.py` "
-                "(there is no fallback implementation)")
+                f"{TRAIN_OPS_PATH} not found: build it with "
+                "`python incagg-gnn_amd/csrc/build_torch_ops.py` (there is no fallback implementation)")
         _train_ops = importlib.import_module("._train_ops", __package__)
     return _train_ops
 
